@@ -76,6 +76,11 @@ SIGNATURES = [
     ("dc_ordered_sum_dev", _i, [_p, _p, _i, _i, _p]),
     ("dc_exp_dev", _i, [_p, _p, _i, _p, _i]),
     ("dc_rmsnorm_dev", _i, [_p, _p, _i, _i, _p, _d, _p, _i]),
+    ("dc_head_norm_rope_dev", _i, [_p, _p]),
+    ("dc_prefix_attention_ws", C.c_size_t, [_p, _p]),
+    ("dc_prefix_attention_dev", _i, [_p, _p, _p, C.c_size_t]),
+    ("dc_cache_weights_dev", _i, [_p, _p]),
+    ("dc_cache_evict_dev", _i, [_p, _p]),
     ("dc_l2_prefetch", _i, [_p, _p, C.c_size_t]),
     ("dc_kernel_probe", _i, [_p, C.POINTER(_u32)]),
     ("dc_fnv1a", _u32, [_p, C.c_size_t]),
@@ -106,6 +111,41 @@ class DcSpec(C.Structure):
     _fields_ = [("hidden", C.c_int), ("layers", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int),
                 ("head_dim", C.c_int), ("inter", C.c_int), ("vocab", C.c_int), ("norm_eps", C.c_double),
                 ("rope_theta", C.c_double), ("tie", C.c_int)]
+
+
+def _fields(pointers: str, longs: str, doubles: str, ints: str):
+    return ([(n, C.c_void_p) for n in pointers.split()] + [(n, C.c_int64) for n in longs.split()]
+            + [(n, C.c_double) for n in doubles.split()] + [(n, C.c_int) for n in ints.split()])
+
+
+class DcHeadRope(C.Structure):
+    """dc_head_rope of include/dcinfer.h."""
+    _fields_ = _fields("x pos slots wq wk inv_freq q k v",
+                       "ldx ld_pos q_row q_head k_seq k_tok k_head v_seq v_tok v_head cache_seqs cache_len",
+                       "eps theta", "rows heads kv_heads head_dim rot axes cyclic x_type out_type") + [
+        ("sections", C.c_int * 4)]
+
+
+class DcPrefixAttn(C.Structure):
+    """dc_prefix_attn of include/dcinfer.h."""
+    _fields_ = _fields("q k_pre v_pre k_own v_own lens out lse",
+                       "q_seq q_row q_head out_seq out_row out_head kp_tok kp_head vp_tok vp_head "
+                       "ko_seq ko_tok ko_head vo_seq vo_tok vo_head", "scale",
+                       "batch rows heads kv_heads head_dim prefix own_max type out_type")
+
+
+class DcCacheWeight(C.Structure):
+    """dc_cache_weight of include/dcinfer.h."""
+    _fields_ = _fields("q k lens lse acc", "q_seq q_row q_head k_seq k_tok k_head acc_seq acc_head", "scale decay",
+                       "batch rows heads kv_heads head_dim cache causal type")
+
+
+class DcCacheEvict(C.Structure):
+    """dc_cache_evict of include/dcinfer.h."""
+    _fields_ = _fields("k v acc lens k_out v_out acc_out index lens_out",
+                       "k_seq k_tok k_head v_seq v_tok v_head acc_seq acc_head ko_seq ko_tok ko_head "
+                       "vo_seq vo_tok vo_head acco_seq acco_head idx_seq idx_head", "",
+                       "batch kv_heads head_dim cache budget recent elem_bytes")
 
 
 def load(path: str | None = None):

@@ -33,6 +33,28 @@ def _ptr(a):
     return C.c_void_p(a.data_ptr())  # torch tensor
 
 
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _type(t) -> int:
+    """The C ABI's name of a tensor's element type (DC_F32, DC_F16, DC_BF16)."""
+    import torch
+    try:
+        return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[t.dtype]
+    except KeyError:
+        raise ValueError(f"element type {t.dtype}: float32, float16 or bfloat16 is needed") from None
+
+
+def _strides(t, what: str) -> list:
+    """The strides of all dimensions but the last, which has to be contiguous; 0 where there is nothing to step over."""
+    s, n = t.stride(), t.shape
+    if n[-1] > 1 and s[-1] != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    return [s[i] if n[i] > 1 else 0 for i in range(len(n) - 1)]
+
+
 def flags_of(d: dict) -> int:
     f = 0
     if d.get("relu"):
@@ -161,6 +183,202 @@ class Compute:
         """infer.js rmsnorm (:70-80) of rows x cols f32 (exact_sum: always the serial-order sum)."""
         self._check(self.L.dc_rmsnorm_dev(self.h, _ptr(x), rows, cols, _ptr(w), float(eps), _ptr(y),
                                           1 if exact_sum else 0), "rmsnorm")
+
+    # ---- a batch's key/value cache (torch CUDA tensors) ---------------------------
+    def _on(self, what: str, **tensors) -> None:
+        for name, t in tensors.items():
+            if t is not None and not (t.is_cuda and t.device.index == self.device):
+                raise ValueError(f"{what}: {name} is not on cuda:{self.device}")
+
+    def _scratch(self, n: int):
+        """n bytes of torch's memory, in the order of the stream that this object launches on."""
+        import torch
+        here = torch.cuda.current_stream(self.device)
+        if (here.cuda_stream or 1) == (self.L.dc_stream(self.h) or 1):
+            return torch.empty(n, dtype=torch.uint8, device=here.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(self.L.dc_stream(self.h), device=self.device)):
+            return torch.empty(n, dtype=torch.uint8, device=here.device)
+
+    def head_norm_rope_dev(self, x, pos, q, k, v, slots=None, *, wq=None, wk=None, eps=1e-5, theta=10000.0,
+                           inv_freq=None, rot=None, sections=None, cyclic: bool = False) -> None:
+        """RMS norm of every query and key head, rotary positions, and the cache
+        append, in one pass over the rows of a fused QKV projection.
+
+        x (rows, (heads + 2 kv_heads) * head_dim) holds [queries | keys | values]
+        of each row (vgemm_dev's output; f32, f16 or bf16).  q (rows, heads,
+        head_dim) receives the queries; k and v, both (slots, kv_heads, head_dim) or
+        (sequences, length, kv_heads, head_dim), the keys and values at slots[row]
+        (int64; a negative one is padding and writes neither; None: row i at slot
+        i).  Slots count through the sequences, and no two rows of a call share one.
+        wq, wk (head_dim, f32): the norm's weights, None for no norm.  pos int32,
+        (rows,) or (axes, rows); sections: pairs of channels that each axis turns,
+        in runs, or with cyclic by turns (pair i on axis i % axes).  rot: channels
+        that are rotated (all); inv_freq (host f64, rot/2) in place of theta.
+        A slot behind the cache is not written and makes the next sync() raise."""
+        _need(x.dim() == 2 and q.dim() == 3 and k.dim() == v.dim() and k.dim() in (3, 4) and k.shape == v.shape,
+              "head_norm_rope: x (rows, width), q (rows, heads, head_dim), k and v (slots.., kv_heads, head_dim)")
+        rows, (heads, D), kv = x.shape[0], q.shape[1:], k.shape[-2]
+        _need(q.shape[0] == rows and k.shape[-1] == D and x.shape[1] == (heads + 2 * kv) * D,
+              f"head_norm_rope: x {tuple(x.shape)}, q {tuple(q.shape)}, k {tuple(k.shape)} do not match")
+        _need(q.dtype == k.dtype == v.dtype, "head_norm_rope: q, k and v are of one type")
+        axes = 1 if pos.dim() == 1 else pos.shape[0]
+        _need(pos.dim() in (1, 2) and pos.shape[-1] == rows and str(pos.dtype) == "torch.int32" and 1 <= axes <= 4,
+              "head_norm_rope: pos is int32 of (rows,) or (1 to 4 axes, rows)")
+        _need(slots is None or (slots.shape == (rows,) and str(slots.dtype) == "torch.int64" and slots.is_contiguous()),
+              "head_norm_rope: slots is int64 of (rows,)")
+        for w in (wq, wk):
+            _need(w is None or (w.shape == (D,) and str(w.dtype) == "torch.float32" and w.is_contiguous()),
+                  "head_norm_rope: wq and wk are f32 of (head_dim,)")
+        rot = D if rot is None else int(rot)
+        sec = [rot // 2] if sections is None else [int(n) for n in sections]
+        _need(len(sec) == axes, f"head_norm_rope: {len(sec)} sections for {axes} position axes")
+        if inv_freq is not None:
+            inv_freq = np.ascontiguousarray(inv_freq, np.float64)
+            _need(inv_freq.shape == (rot // 2,), "head_norm_rope: inv_freq has rot/2 values")
+        self._on("head_norm_rope", x=x, pos=pos, q=q, k=k, v=v, slots=slots, wq=wq, wk=wk)
+        sx, sq, sp = _strides(x, "x")[0], _strides(q, "q"), _strides(pos, "pos")
+        sk, sv = _strides(k, "k"), _strides(v, "v")
+        seqs, length = (1, k.shape[0]) if k.dim() == 3 else k.shape[:2]
+        if k.dim() == 3:
+            sk, sv = [0] + sk, [0] + sv
+        a = _lib.DcHeadRope(
+            x.data_ptr(), pos.data_ptr(), slots.data_ptr() if slots is not None else None,
+            wq.data_ptr() if wq is not None else None, wk.data_ptr() if wk is not None else None,
+            inv_freq.ctypes.data if inv_freq is not None else None, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            sx if rows > 1 else x.shape[1], sp[0] if sp and axes > 1 else rows, sq[0], sq[1], *sk, *sv, seqs, length,
+            eps, theta, rows, heads, kv, D, rot, axes, 1 if cyclic else 0, _type(x), _type(q),
+            (C.c_int * 4)(*sec))
+        self._check(self.L.dc_head_norm_rope_dev(self.h, C.byref(a)), "head_norm_rope")
+
+    def prefix_attention_dev(self, q, out, k_pre=None, v_pre=None, k_own=None, v_own=None, lens=None, lse=None, *,
+                             scale=None, ws=None) -> None:
+        """Attention of a batch over a prefix that its sequences share, computed for
+        all of them in one pass over the prefix, and over each one's own cache.
+
+        q (batch, rows, heads, head_dim), f16 or bf16, up to 16 rows a sequence (a
+        decode step's token, or a token and its drafts); k_pre, v_pre (tokens,
+        kv_heads, head_dim): seen by every row; k_own, v_own (batch, length,
+        kv_heads, head_dim) with lens (batch, int32, on the device): row r of
+        sequence b sees the first lens[b] - (rows - 1 - r) tokens, so a row sees
+        itself and what came before.  Either pair may be left out.  out (as q, or
+        f32) and lse (batch, rows, heads, f32; optional): softmax(scale q k) v and
+        log(sum(exp(scale q k))), 0 and -inf for a row that sees nothing.  scale:
+        1/sqrt(head_dim) unless given.  ws: workspace (prefix_attention_ws bytes)
+        for callers that hold their own; otherwise torch's allocator gives it."""
+        a = self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale)
+        n = self.L.dc_prefix_attention_ws(self.h, C.byref(a))
+        if ws is None:
+            ws = self._scratch(n) if n else None
+        else:
+            self._on("prefix_attention", ws=ws)
+            _need(ws.is_contiguous(), "prefix_attention: ws is contiguous")
+        self._check(self.L.dc_prefix_attention_dev(self.h, C.byref(a), ws.data_ptr() if ws is not None else None,
+                                                   ws.numel() * ws.element_size() if ws is not None else 0),
+                    "prefix_attention")
+
+    def prefix_attention_ws(self, q, out, k_pre=None, v_pre=None, k_own=None, v_own=None, lens=None, lse=None, *,
+                            scale=None) -> int:
+        """Bytes of workspace that prefix_attention_dev takes for these arguments (their sizes alone count)."""
+        a = self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale)
+        return self.L.dc_prefix_attention_ws(self.h, C.byref(a))
+
+    def _prefix_attn(self, q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale):
+        _need(q.dim() == 4 and out.shape == q.shape, "prefix_attention: q and out are (batch, rows, heads, head_dim)")
+        B, R, heads, D = q.shape
+        _need((k_pre is None) == (v_pre is None) and (k_own is None) == (v_own is None) == (lens is None),
+              "prefix_attention: k_pre comes with v_pre, k_own with v_own and lens")
+        some = k_pre if k_pre is not None else k_own
+        kv = some.shape[-2] if some is not None else heads
+        sp, so, prefix, own_max = [0] * 4, [0] * 6, 0, 0
+        if k_pre is not None:
+            prefix = k_pre.shape[0]
+            _need(k_pre.shape == v_pre.shape == (prefix, kv, D) and k_pre.dtype == v_pre.dtype == q.dtype,
+                  "prefix_attention: k_pre and v_pre are (tokens, kv_heads, head_dim) of q's type")
+            sp = _strides(k_pre, "k_pre") + _strides(v_pre, "v_pre")
+        if k_own is not None:
+            own_max = k_own.shape[1] if k_own.dim() == 4 else 0
+            _need(k_own.shape == v_own.shape == (B, own_max, kv, D) and k_own.dtype == v_own.dtype == q.dtype,
+                  "prefix_attention: k_own and v_own are (batch, length, kv_heads, head_dim) of q's type")
+            _need(lens.shape == (B,) and str(lens.dtype) == "torch.int32" and lens.is_contiguous(),
+                  "prefix_attention: lens is int32 of (batch,)")
+            so = _strides(k_own, "k_own") + _strides(v_own, "v_own")
+        _need(lse is None or (lse.shape == (B, R, heads) and str(lse.dtype) == "torch.float32" and lse.is_contiguous()),
+              "prefix_attention: lse is f32 of (batch, rows, heads)")
+        self._on("prefix_attention", q=q, out=out, k_pre=k_pre, v_pre=v_pre, k_own=k_own, v_own=v_own, lens=lens,
+                 lse=lse)
+        p = [t.data_ptr() if t is not None else None for t in (q, k_pre, v_pre, k_own, v_own, lens, out, lse)]
+        return _lib.DcPrefixAttn(*p, *_strides(q, "q"), *_strides(out, "out"), *sp, *so,
+                                 D ** -0.5 if scale is None else scale, B, R, heads, kv, D, prefix, own_max, _type(q),
+                                 _type(out))
+
+    def cache_weights_dev(self, q, k, lens, lse, acc, *, scale=None, decay: float = 1.0, causal: bool = True) -> None:
+        """Adds to acc (batch, kv_heads, length, f32) the softmax weight that every
+        cached key receives from these queries: acc = decay * acc + the sum over
+        rows and heads of a group of exp(scale q k - lse), for the first lens[b]
+        tokens of sequence b; the rest of acc stays.
+
+        q (batch, rows, heads, head_dim), k (batch, length, kv_heads, head_dim), f16
+        or bf16; lens (batch, int32) and lse (batch, rows, heads, f32) as
+        prefix_attention_dev takes and gives them (with a prefix, lse spans both).
+        causal: row r sees lens[b] - (rows - 1 - r) tokens; False: all rows see all
+        (the shared prefix: its k as one sequence, all rows of the batch as rows).
+        decay 0 overwrites."""
+        _need(q.dim() == 4 and k.dim() == 4 and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3]
+              and q.dtype == k.dtype,
+              "cache_weights: q (batch, rows, heads, head_dim), k (batch, length, kv_heads, head_dim) of one type")
+        B, R, heads, D = q.shape
+        L, kv = k.shape[1:3]
+        _need(acc.shape == (B, kv, L) and str(acc.dtype) == "torch.float32",
+              "cache_weights: acc is f32 of (batch, kv_heads, length)")
+        _need(lens.shape == (B,) and str(lens.dtype) == "torch.int32" and lens.is_contiguous(),
+              "cache_weights: lens is int32 of (batch,)")
+        _need(lse.shape == (B, R, heads) and str(lse.dtype) == "torch.float32" and lse.is_contiguous(),
+              "cache_weights: lse is f32 of (batch, rows, heads)")
+        self._on("cache_weights", q=q, k=k, lens=lens, lse=lse, acc=acc)
+        a = _lib.DcCacheWeight(q.data_ptr(), k.data_ptr(), lens.data_ptr(), lse.data_ptr(), acc.data_ptr(),
+                               *_strides(q, "q"), *_strides(k, "k"), *_strides(acc, "acc"),
+                               D ** -0.5 if scale is None else scale, decay, B, R, heads, kv, D, L,
+                               1 if causal else 0, _type(q))
+        self._check(self.L.dc_cache_weights_dev(self.h, C.byref(a)), "cache_weights")
+
+    def cache_evict_dev(self, k, v, acc, lens, k_out, v_out, acc_out, index, lens_out, *, budget: int,
+                        recent: int = 0) -> None:
+        """Writes the kept tokens of a batch's cache to another one, for each
+        sequence and key/value head: all where lens[b] <= budget, else the last
+        `recent` and, of those before, the budget - recent of largest acc (equal
+        ones: the lower index; a NaN is the lowest), in their order.
+
+        k, v (batch, length, kv_heads, head_dim) and acc (batch, kv_heads, length,
+        f32); k_out, v_out, acc_out and index (batch, kv_heads, .., int32: each kept
+        token's old place) alike, with room for `budget` tokens; lens, lens_out
+        (batch, int32).  What lies behind a sequence's last kept token is left as
+        it is.  Heads keep different tokens but equally many.  The outputs must not
+        overlap the inputs."""
+        budget, recent = int(budget), int(recent)
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
+              "cache_evict: k and v are (batch, length, kv_heads, head_dim) of one type")
+        B, L, kv, D = k.shape
+        room = min(budget, L)
+        _need(k_out.shape == v_out.shape and k_out.dim() == 4 and k_out.dtype == v_out.dtype == k.dtype
+              and (k_out.shape[0], *k_out.shape[2:]) == (B, kv, D) and k_out.shape[1] >= room,
+              "cache_evict: k_out and v_out are as k, with room for the budget")
+        for name, t, kind in (("acc", acc, "torch.float32"), ("acc_out", acc_out, "torch.float32"),
+                              ("index", index, "torch.int32")):
+            _need(t.dim() == 3 and t.shape[:2] == (B, kv) and str(t.dtype) == kind
+                  and (t.shape[2] == L if name == "acc" else t.shape[2] >= room),
+                  f"cache_evict: {name} is {kind[6:]} of (batch, kv_heads, tokens)")
+        for name, t in (("lens", lens), ("lens_out", lens_out)):
+            _need(t.shape == (B,) and str(t.dtype) == "torch.int32" and t.is_contiguous(),
+                  f"cache_evict: {name} is int32 of (batch,)")
+        self._on("cache_evict", k=k, v=v, acc=acc, lens=lens, k_out=k_out, v_out=v_out, acc_out=acc_out, index=index,
+                 lens_out=lens_out)
+        _type(k)
+        a = _lib.DcCacheEvict(
+            *(t.data_ptr() for t in (k, v, acc, lens, k_out, v_out, acc_out, index, lens_out)),
+            *_strides(k, "k"), *_strides(v, "v"), *_strides(acc, "acc"), *_strides(k_out, "k_out"),
+            *_strides(v_out, "v_out"), *_strides(acc_out, "acc_out"), *_strides(index, "index"),
+            B, kv, D, L, budget, recent, k.element_size())
+        self._check(self.L.dc_cache_evict_dev(self.h, C.byref(a)), "cache_evict")
 
     def measure_capacity(self, spec=None, T: int = 16, seconds: float = 0.3) -> float:
         """The capacity the ring's planner apportions layers by, in the

@@ -1,0 +1,109 @@
+// dc_cache.cuh -- what the cache operators share: types, spans of strided
+// buffers (argument checks) and the launch.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <initializer_list>
+
+#include "dc_internal.cuh"
+#include "dc_ptx.cuh"
+
+namespace dcc {
+
+static inline bool is_type(int t) { return t == DC_F32 || t == DC_F16 || t == DC_BF16; }
+static inline bool is_half(int t) { return t == DC_F16 || t == DC_BF16; }
+static inline int elem_size(int t) { return t == DC_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// The addresses that a strided buffer covers, from its first to behind its
+// last byte, for the overlap checks.
+struct Dim {
+  int64_t n, stride;
+};
+struct Span {
+  uintptr_t lo = 0, hi = 0;
+  bool ok = true;
+  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+static inline Span span(const void* p, int elem, std::initializer_list<Dim> dims) {
+  Span s;
+  if (!p) return s;
+  int64_t last = 0;
+  bool empty = false;
+  for (const Dim& d : dims) {
+    if (d.stride < 0) s.ok = false;
+    if (d.n <= 0) empty = true;
+    else last += (d.n - 1) * d.stride;
+  }
+  if (empty || !s.ok) return s;
+  s.lo = (uintptr_t)p;
+  s.hi = s.lo + (uintptr_t)(last + 1) * elem;
+  return s;
+}
+// Whether a buffer of es-byte elements begins, and each of its rows (at these
+// strides), on a boundary of `align` bytes.
+static inline bool aligned(const void* p, int es, int align, std::initializer_list<int64_t> strides) {
+  uintptr_t m = (uintptr_t)p;
+  for (int64_t s : strides) m |= (uintptr_t)(s * es);
+  return !(m & (align - 1));
+}
+
+// A call may come while another device is current: launches and kernel
+// attributes belong to the context's own.
+struct DeviceGuard {
+  int old = -1;
+  int enter(dc_ctx* ctx) {
+    int cur = -1;
+    DC_CUDA(ctx, cudaGetDevice(&cur));
+    if (cur != ctx->device) {
+      DC_CUDA(ctx, cudaSetDevice(ctx->device));
+      old = cur;
+    }
+    return DC_OK;
+  }
+  ~DeviceGuard() {
+    if (old >= 0) cudaSetDevice(old);
+  }
+};
+
+// One launch on the context's stream, in clusters of `cluster` blocks along x,
+// as a programmatic dependent of what runs before: every kernel here executes
+// griddepcontrol.wait before it touches memory.
+template <typename... P, typename... A>
+static int launch(dc_ctx* ctx, void (*kern)(P...), dim3 grid, int threads, int smem, int cluster, const A&... args) {
+  if (int rc = dc_set_smem(ctx, (const void*)kern, smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  cfg.attrs = attr;
+  DC_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, args...));
+  dc_count_launch();
+  return DC_OK;
+}
+
+}  // namespace dcc

@@ -179,6 +179,123 @@ int dc_exp_dev(dc_ctx* ctx, const double* x, int n, double* y, int sel);
 int dc_rmsnorm_dev(dc_ctx* ctx, const float* x, int rows, int cols, const float* w, double eps, float* y,
                    int exact_sum);
 
+/* ---- a batch's key/value cache, device buffers --------------------------------
+ * What a batch of sequences needs between its QKV and its O projection
+ * (dc_vgemm): the rotated heads and the cache rows, attention over a prefix
+ * that all sequences share and over each sequence's own keys, the weight every
+ * cached key receives, and a cache without the keys of least weight.  (No
+ * counterpart in the reference, which keeps one sequence's cache per stage.)
+ * Types are DC_F32 / DC_F16 / DC_BF16; strides are in elements, the last
+ * dimension (head_dim) is contiguous.  All calls are asynchronous on the
+ * context's stream, allocate nothing, and may be captured into a graph.  A buffer
+ * that a call writes lies apart from those it reads and writes besides. */
+#define DC_F32 0
+#define DC_F16 1
+#define DC_BF16 2
+#define DC_MAX_AXES 4
+#define DC_MAX_ROT 256
+
+/* dc_head_norm_rope_dev: x holds rows of [heads queries | kv_heads keys |
+ * kv_heads values], each head_dim wide, ldx apart.  Every query and key head is
+ * normalised, y = x / sqrt(mean(x^2) + eps) * w (skipped where wq / wk is
+ * NULL), and its first `rot` channels are rotated: with (lo, hi) = (y[i],
+ * y[i + rot/2]) and the angle t_i = position * theta^(-2i/rot), lo' = lo cos t -
+ * hi sin t, hi' = hi cos t + lo sin t.  Positions are pos[axis * ld_pos + row];
+ * pair i takes the axis that `sections` gives it (sections[0..axes) pairs, rot/2
+ * in all): runs in order of the axes, or (cyclic = 1) pair i the axis i % axes
+ * while i / axes < sections[i % axes], else axis 0.  inv_freq (host, rot/2
+ * doubles, or NULL) replaces theta^(-2i/rot).  Angles are formed in 64 bits, the
+ * norm and the rotation in 32, each output rounded once.
+ * Query heads go to q[row * q_row + head * q_head].  Keys and values go to cache
+ * slot slots[row] (int64, or NULL: the row's own number): slot s is token s %
+ * cache_len of sequence s / cache_len, at token * k_tok + sequence * k_seq + head
+ * * k_head.  A row of negative slot writes no key or value (padding); a slot of
+ * cache_seqs * cache_len or more is not written either and dc_sync reports it.
+ * Slots of one call are distinct.  head_dim and rot are multiples of 8,
+ * head_dim <= 256. */
+typedef struct dc_head_rope {
+  const void* x;
+  const int32_t* pos;
+  const int64_t* slots;
+  const float *wq, *wk;
+  const double* inv_freq;
+  void *q, *k, *v;
+  int64_t ldx, ld_pos, q_row, q_head, k_seq, k_tok, k_head, v_seq, v_tok, v_head, cache_seqs, cache_len;
+  double eps, theta;
+  int rows, heads, kv_heads, head_dim, rot, axes, cyclic, x_type, out_type;
+  int sections[DC_MAX_AXES];
+} dc_head_rope;
+int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* a);
+
+/* dc_prefix_attention_dev: row r of sequence b attends to all `prefix` tokens of
+ * k_pre / v_pre, which the batch shares, and to the first lens[b] - (rows - 1 -
+ * r) tokens of its own cache k_own / v_own (sequence b of it; own_max tokens;
+ * lens is device memory and already counts the rows' own tokens):
+ *   out = softmax(scale * q K^T) V,   lse = log(sum(exp(scale * q K^T)))
+ * over the two together, query head h with key/value head h / (heads /
+ * kv_heads).  lens[b] is taken as at most own_max and at least 0; a row that
+ * sees nothing, or nothing but scores of -inf, has out 0 and lse -inf.  What lies
+ * behind a row's tokens is not looked at: it may hold anything, NaN too.
+ * type (q, k, v) is DC_F16 or DC_BF16, out_type that or DC_F32; softmax statistics
+ * and sums are f32, the probabilities are rounded to `type` for the product with
+ * v.  rows <= 16; head_dim a multiple of 8, <= 128; q, k, v and out rows begin on
+ * 16-byte boundaries.  ws: dc_prefix_attention_ws bytes of device memory
+ * (16-byte aligned) that no other call uses at the same time. */
+typedef struct dc_prefix_attn {
+  const void *q, *k_pre, *v_pre, *k_own, *v_own;
+  const int32_t* lens;
+  void* out;
+  float* lse; /* batch x rows x heads, or NULL */
+  int64_t q_seq, q_row, q_head, out_seq, out_row, out_head;
+  int64_t kp_tok, kp_head, vp_tok, vp_head, ko_seq, ko_tok, ko_head, vo_seq, vo_tok, vo_head;
+  double scale;
+  int batch, rows, heads, kv_heads, head_dim, prefix, own_max, type, out_type;
+} dc_prefix_attn;
+size_t dc_prefix_attention_ws(const dc_ctx* ctx, const dc_prefix_attn* a);
+int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* a, void* ws, size_t ws_bytes);
+
+/* dc_cache_weights_dev: the softmax weight that the tokens of each sequence's
+ * cache receive from its query rows, accumulated in place for each key/value head:
+ *   acc[b][g][j] = decay * acc[b][g][j] + sum over rows r, heads h of g of
+ *                  exp(scale * q[b][r][h] . k[b][j][g] - lse[b][r][h])
+ * for j < lens[b] (clamped to [0, cache]); the rest of acc is left as it is.
+ * causal = 1: row r sees tokens j < lens[b] - (rows - 1 - r), as above; 0: all
+ * rows see all tokens (a shared prefix: batch 1, the batch's rows as rows).
+ * decay = 0 overwrites without reading acc; a row of lse -inf adds nothing.  The
+ * sum's order is fixed: equal inputs give equal bits.  Types and alignment as
+ * above; heads / kv_heads <= 128. */
+typedef struct dc_cache_weight {
+  const void *q, *k;
+  const int32_t* lens;
+  const float* lse; /* batch x rows x heads */
+  float* acc;
+  int64_t q_seq, q_row, q_head, k_seq, k_tok, k_head, acc_seq, acc_head;
+  double scale, decay;
+  int batch, rows, heads, kv_heads, head_dim, cache, causal, type;
+} dc_cache_weight;
+int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* a);
+
+/* dc_cache_evict_dev: writes, for each sequence and key/value head, the tokens of
+ * a cache that are kept, in their order, to another cache.  Of n = lens[b]
+ * (clamped to [0, cache]) tokens all are kept when n <= budget; otherwise the
+ * last `recent`, and of those before them the budget - recent of largest acc
+ * (equal ones: the lower index; NaN counts as the lowest).  index receives each
+ * kept token's place in the old cache, acc_out its acc, lens_out[b] = min(n,
+ * budget); places behind that are left as they are.  elem_bytes (k, v) is 2 or 4;
+ * k and v rows are multiples of 16 bytes and begin on 16-byte boundaries. */
+typedef struct dc_cache_evict {
+  const void *k, *v;
+  const float* acc;
+  const int32_t* lens;
+  void *k_out, *v_out;
+  float* acc_out;
+  int32_t *index, *lens_out;
+  int64_t k_seq, k_tok, k_head, v_seq, v_tok, v_head, acc_seq, acc_head;
+  int64_t ko_seq, ko_tok, ko_head, vo_seq, vo_tok, vo_head, acco_seq, acco_head, idx_seq, idx_head;
+  int batch, kv_heads, head_dim, cache, budget, recent, elem_bytes;
+} dc_cache_evict;
+int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* a);
+
 /* Prefetch [p, p + bytes) of device memory into L2 (16-byte aligned range),
  * asynchronously on the context's stream.  No counterpart in the reference; a
  * host may warm a buffer it is about to use (the stage forward does not call
