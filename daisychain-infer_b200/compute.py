@@ -33,28 +33,6 @@ def _ptr(a):
     return C.c_void_p(a.data_ptr())  # torch tensor
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _type(t) -> int:
-    """The C ABI's name of a tensor's element type (DC_F32, DC_F16, DC_BF16)."""
-    import torch
-    try:
-        return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[t.dtype]
-    except KeyError:
-        raise ValueError(f"element type {t.dtype}: float32, float16 or bfloat16 is needed") from None
-
-
-def _strides(t, what: str) -> list:
-    """The strides of all dimensions but the last, which has to be contiguous; 0 where there is nothing to step over."""
-    s, n = t.stride(), t.shape
-    if n[-1] > 1 and s[-1] != 1:
-        raise ValueError(f"{what}: the last dimension must be contiguous")
-    return [s[i] if n[i] > 1 else 0 for i in range(len(n) - 1)]
-
-
 def flags_of(d: dict) -> int:
     f = 0
     if d.get("relu"):
@@ -185,18 +163,35 @@ class Compute:
                                           1 if exact_sum else 0), "rmsnorm")
 
     # ---- a batch's key/value cache (torch CUDA tensors) ---------------------------
-    def _on(self, what: str, **tensors) -> None:
-        for name, t in tensors.items():
-            if t is not None and not (t.is_cuda and t.device.index == self.device):
-                raise ValueError(f"{what}: {name} is not on cuda:{self.device}")
+    def _types(self) -> dict:
+        """torch's element types by the C ABI's names (DC_F32, DC_F16, DC_BF16)."""
+        t = Compute._type_of
+        if not t:
+            import torch
+            t.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, "i32": torch.int32, "i64": torch.int64})
+        return t
+
+    _type_of: dict = {}
+
+    def _ptrs(self, what: str, *tensors) -> list:
+        """The tensors' addresses (0 for None), all on this object's device."""
+        for t in tensors:
+            if t is not None and t.get_device() != self.device:
+                raise ValueError(f"{what}: a tensor is not on cuda:{self.device}")
+        return [t.data_ptr() if t is not None else 0 for t in tensors]
+
+    @staticmethod
+    def _flat(t, shape, dtype) -> bool:
+        return t.shape == shape and t.dtype is dtype and t.is_contiguous()
 
     def _scratch(self, n: int):
         """n bytes of torch's memory, in the order of the stream that this object launches on."""
         import torch
         here = torch.cuda.current_stream(self.device)
-        if (here.cuda_stream or 1) == (self.L.dc_stream(self.h) or 1):
+        stream = self.L.dc_stream(self.h)
+        if (here.cuda_stream or 1) == (stream or 1):
             return torch.empty(n, dtype=torch.uint8, device=here.device)
-        with torch.cuda.stream(torch.cuda.ExternalStream(self.L.dc_stream(self.h), device=self.device)):
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
             return torch.empty(n, dtype=torch.uint8, device=here.device)
 
     def head_norm_rope_dev(self, x, pos, q, k, v, slots=None, *, wq=None, wk=None, eps=1e-5, theta=10000.0,
@@ -215,40 +210,47 @@ class Compute:
         in runs, or with cyclic by turns (pair i on axis i % axes).  rot: channels
         that are rotated (all); inv_freq (host f64, rot/2) in place of theta.
         A slot behind the cache is not written and makes the next sync() raise."""
-        _need(x.dim() == 2 and q.dim() == 3 and k.dim() == v.dim() and k.dim() in (3, 4) and k.shape == v.shape,
-              "head_norm_rope: x (rows, width), q (rows, heads, head_dim), k and v (slots.., kv_heads, head_dim)")
-        rows, (heads, D), kv = x.shape[0], q.shape[1:], k.shape[-2]
-        _need(q.shape[0] == rows and k.shape[-1] == D and x.shape[1] == (heads + 2 * kv) * D,
-              f"head_norm_rope: x {tuple(x.shape)}, q {tuple(q.shape)}, k {tuple(k.shape)} do not match")
-        _need(q.dtype == k.dtype == v.dtype, "head_norm_rope: q, k and v are of one type")
-        axes = 1 if pos.dim() == 1 else pos.shape[0]
-        _need(pos.dim() in (1, 2) and pos.shape[-1] == rows and str(pos.dtype) == "torch.int32" and 1 <= axes <= 4,
-              "head_norm_rope: pos is int32 of (rows,) or (1 to 4 axes, rows)")
-        _need(slots is None or (slots.shape == (rows,) and str(slots.dtype) == "torch.int64" and slots.is_contiguous()),
-              "head_norm_rope: slots is int64 of (rows,)")
+        T = self._types()
+        if x.ndim != 2 or q.ndim != 3 or k.ndim not in (3, 4) or v.shape != k.shape:
+            raise ValueError("head_norm_rope: x (rows, width), q (rows, heads, head_dim), k and v (slots.., kv_heads, "
+                             "head_dim)")
+        rows, width = x.shape
+        rows_q, heads, D = q.shape
+        seqs, (length, kv, Dk) = (1, k.shape) if k.ndim == 3 else (k.shape[0], k.shape[1:])
+        if rows_q != rows or Dk != D or width != (heads + 2 * kv) * D:
+            raise ValueError(f"head_norm_rope: x {tuple(x.shape)}, q {tuple(q.shape)}, k {tuple(k.shape)} do not match")
+        dt = q.dtype
+        if k.dtype is not dt or v.dtype is not dt or dt not in T or x.dtype not in T:
+            raise ValueError("head_norm_rope: x, and q, k and v of one type: float32, float16 or bfloat16")
+        axes, npos = (1, pos.shape[0]) if pos.ndim == 1 else pos.shape if pos.ndim == 2 else (0, 0)
+        if npos != rows or pos.dtype is not T["i32"] or not 1 <= axes <= 4:
+            raise ValueError("head_norm_rope: pos is int32 of (rows,) or (1 to 4 axes, rows)")
+        if slots is not None and not self._flat(slots, (rows,), T["i64"]):
+            raise ValueError("head_norm_rope: slots is int64 of (rows,)")
         for w in (wq, wk):
-            _need(w is None or (w.shape == (D,) and str(w.dtype) == "torch.float32" and w.is_contiguous()),
-                  "head_norm_rope: wq and wk are f32 of (head_dim,)")
+            if w is not None and not (T.get(w.dtype) == 0 and w.shape == (D,) and w.is_contiguous()):
+                raise ValueError("head_norm_rope: wq and wk are f32 of (head_dim,)")
         rot = D if rot is None else int(rot)
         sec = [rot // 2] if sections is None else [int(n) for n in sections]
-        _need(len(sec) == axes, f"head_norm_rope: {len(sec)} sections for {axes} position axes")
+        if len(sec) != axes:
+            raise ValueError(f"head_norm_rope: {len(sec)} sections for {axes} position axes")
+        freq = 0
         if inv_freq is not None:
             inv_freq = np.ascontiguousarray(inv_freq, np.float64)
-            _need(inv_freq.shape == (rot // 2,), "head_norm_rope: inv_freq has rot/2 values")
-        self._on("head_norm_rope", x=x, pos=pos, q=q, k=k, v=v, slots=slots, wq=wq, wk=wk)
-        sx, sq, sp = _strides(x, "x")[0], _strides(q, "q"), _strides(pos, "pos")
-        sk, sv = _strides(k, "k"), _strides(v, "v")
-        seqs, length = (1, k.shape[0]) if k.dim() == 3 else k.shape[:2]
-        if k.dim() == 3:
-            sk, sv = [0] + sk, [0] + sv
-        a = _lib.DcHeadRope(
-            x.data_ptr(), pos.data_ptr(), slots.data_ptr() if slots is not None else None,
-            wq.data_ptr() if wq is not None else None, wk.data_ptr() if wk is not None else None,
-            inv_freq.ctypes.data if inv_freq is not None else None, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            sx if rows > 1 else x.shape[1], sp[0] if sp and axes > 1 else rows, sq[0], sq[1], *sk, *sv, seqs, length,
-            eps, theta, rows, heads, kv, D, rot, axes, 1 if cyclic else 0, _type(x), _type(q),
-            (C.c_int * 4)(*sec))
-        self._check(self.L.dc_head_norm_rope_dev(self.h, C.byref(a)), "head_norm_rope")
+            if inv_freq.shape != (rot // 2,):
+                raise ValueError("head_norm_rope: inv_freq has rot/2 values")
+            freq = inv_freq.ctypes.data
+        sx, sp, sq, sk, sv = x.stride(), pos.stride(), q.stride(), k.stride(), v.stride()
+        if (sx[-1], sp[-1] if rows > 1 else 1, sq[-1], sk[-1], sv[-1]) != (1, 1, 1, 1, 1):
+            raise ValueError("head_norm_rope: the last dimension of x, pos, q, k and v must be contiguous")
+        px, pp, ps, pwq, pwk, pq, pk, pv = self._ptrs("head_norm_rope", x, pos, slots, wq, wk, q, k, v)
+        a = _lib.HEAD_ROPE.pack(
+            px, pp, ps, pwq, pwk, freq, pq, pk, pv, sx[0], sp[0] if axes > 1 else rows, sq[0], sq[1],
+            *((0, *sk[:2], 0, *sv[:2]) if k.ndim == 3 else (*sk[:3], *sv[:3])), seqs, length, eps, theta, rows, heads,
+            kv, D, rot, axes, 1 if cyclic else 0, T[x.dtype], T[dt], *sec, *(0,) * (4 - axes))
+        rc = self.L.dc_head_norm_rope_dev(self.h, a)
+        if rc:
+            self._check(rc, "head_norm_rope")
 
     def prefix_attention_dev(self, q, out, k_pre=None, v_pre=None, k_own=None, v_own=None, lens=None, lse=None, *,
                              scale=None, ws=None) -> None:
@@ -266,50 +268,58 @@ class Compute:
         1/sqrt(head_dim) unless given.  ws: workspace (prefix_attention_ws bytes)
         for callers that hold their own; otherwise torch's allocator gives it."""
         a = self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale)
-        n = self.L.dc_prefix_attention_ws(self.h, C.byref(a))
         if ws is None:
+            n = self.L.dc_prefix_attention_ws(self.h, a)
             ws = self._scratch(n) if n else None
-        else:
-            self._on("prefix_attention", ws=ws)
-            _need(ws.is_contiguous(), "prefix_attention: ws is contiguous")
-        self._check(self.L.dc_prefix_attention_dev(self.h, C.byref(a), ws.data_ptr() if ws is not None else None,
-                                                   ws.numel() * ws.element_size() if ws is not None else 0),
-                    "prefix_attention")
+        elif not ws.is_contiguous():
+            raise ValueError("prefix_attention: ws is contiguous")
+        at, = self._ptrs("prefix_attention", ws)
+        rc = self.L.dc_prefix_attention_dev(self.h, a, at, ws.numel() * ws.element_size() if at else 0)
+        if rc:
+            self._check(rc, "prefix_attention")
 
     def prefix_attention_ws(self, q, out, k_pre=None, v_pre=None, k_own=None, v_own=None, lens=None, lse=None, *,
                             scale=None) -> int:
         """Bytes of workspace that prefix_attention_dev takes for these arguments (their sizes alone count)."""
-        a = self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale)
-        return self.L.dc_prefix_attention_ws(self.h, C.byref(a))
+        return self.L.dc_prefix_attention_ws(
+            self.h, self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale))
 
-    def _prefix_attn(self, q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale):
-        _need(q.dim() == 4 and out.shape == q.shape, "prefix_attention: q and out are (batch, rows, heads, head_dim)")
+    def _prefix_attn(self, q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale) -> bytes:
+        T = self._types()
+        dt = q.dtype
+        if q.ndim != 4 or out.shape != q.shape or dt not in T or out.dtype not in T:
+            raise ValueError("prefix_attention: q and out are (batch, rows, heads, head_dim), f16 or bf16 (out also f32)")
         B, R, heads, D = q.shape
-        _need((k_pre is None) == (v_pre is None) and (k_own is None) == (v_own is None) == (lens is None),
-              "prefix_attention: k_pre comes with v_pre, k_own with v_own and lens")
-        some = k_pre if k_pre is not None else k_own
-        kv = some.shape[-2] if some is not None else heads
-        sp, so, prefix, own_max = [0] * 4, [0] * 6, 0, 0
+        if (k_pre is None) != (v_pre is None) or not (k_own is None) == (v_own is None) == (lens is None):
+            raise ValueError("prefix_attention: k_pre comes with v_pre, k_own with v_own and lens")
+        sq, so = q.stride(), out.stride()
+        last = sq[3] == 1 and so[3] == 1
+        kv = k_pre.shape[-2] if k_pre is not None else k_own.shape[-2] if k_own is not None else heads
+        pre, own, prefix, own_max = (0,) * 4, (0,) * 6, 0, 0
         if k_pre is not None:
             prefix = k_pre.shape[0]
-            _need(k_pre.shape == v_pre.shape == (prefix, kv, D) and k_pre.dtype == v_pre.dtype == q.dtype,
-                  "prefix_attention: k_pre and v_pre are (tokens, kv_heads, head_dim) of q's type")
-            sp = _strides(k_pre, "k_pre") + _strides(v_pre, "v_pre")
+            if k_pre.shape != (prefix, kv, D) or v_pre.shape != k_pre.shape or k_pre.dtype is not dt or (
+                    v_pre.dtype is not dt):
+                raise ValueError("prefix_attention: k_pre and v_pre are (tokens, kv_heads, head_dim) of q's type")
+            a, b, c = k_pre.stride()
+            d, e, f = v_pre.stride()
+            pre, last = (a, b, d, e), last and c == 1 and f == 1
         if k_own is not None:
-            own_max = k_own.shape[1] if k_own.dim() == 4 else 0
-            _need(k_own.shape == v_own.shape == (B, own_max, kv, D) and k_own.dtype == v_own.dtype == q.dtype,
-                  "prefix_attention: k_own and v_own are (batch, length, kv_heads, head_dim) of q's type")
-            _need(lens.shape == (B,) and str(lens.dtype) == "torch.int32" and lens.is_contiguous(),
-                  "prefix_attention: lens is int32 of (batch,)")
-            so = _strides(k_own, "k_own") + _strides(v_own, "v_own")
-        _need(lse is None or (lse.shape == (B, R, heads) and str(lse.dtype) == "torch.float32" and lse.is_contiguous()),
-              "prefix_attention: lse is f32 of (batch, rows, heads)")
-        self._on("prefix_attention", q=q, out=out, k_pre=k_pre, v_pre=v_pre, k_own=k_own, v_own=v_own, lens=lens,
-                 lse=lse)
-        p = [t.data_ptr() if t is not None else None for t in (q, k_pre, v_pre, k_own, v_own, lens, out, lse)]
-        return _lib.DcPrefixAttn(*p, *_strides(q, "q"), *_strides(out, "out"), *sp, *so,
-                                 D ** -0.5 if scale is None else scale, B, R, heads, kv, D, prefix, own_max, _type(q),
-                                 _type(out))
+            own_max = k_own.shape[1] if k_own.ndim == 4 else 0
+            if k_own.shape != (B, own_max, kv, D) or v_own.shape != k_own.shape or k_own.dtype is not dt or (
+                    v_own.dtype is not dt):
+                raise ValueError("prefix_attention: k_own and v_own are (batch, length, kv_heads, head_dim) of q's type")
+            if not self._flat(lens, (B,), T["i32"]):
+                raise ValueError("prefix_attention: lens is int32 of (batch,)")
+            a, b, c = k_own.stride(), v_own.stride(), last
+            own, last = (*a[:3], *b[:3]), last and a[3] == 1 and b[3] == 1
+        if not last:
+            raise ValueError("prefix_attention: the last dimension of q, k, v and out must be contiguous")
+        if lse is not None and not (T.get(lse.dtype) == 0 and lse.shape == (B, R, heads) and lse.is_contiguous()):
+            raise ValueError("prefix_attention: lse is f32 of (batch, rows, heads)")
+        return _lib.PREFIX_ATTN.pack(
+            *self._ptrs("prefix_attention", q, k_pre, v_pre, k_own, v_own, lens, out, lse), *sq[:3], *so[:3], *pre,
+            *own, D ** -0.5 if scale is None else scale, B, R, heads, kv, D, prefix, own_max, T[dt], T[out.dtype])
 
     def cache_weights_dev(self, q, k, lens, lse, acc, *, scale=None, decay: float = 1.0, causal: bool = True) -> None:
         """Adds to acc (batch, kv_heads, length, f32) the softmax weight that every
@@ -323,23 +333,28 @@ class Compute:
         causal: row r sees lens[b] - (rows - 1 - r) tokens; False: all rows see all
         (the shared prefix: its k as one sequence, all rows of the batch as rows).
         decay 0 overwrites."""
-        _need(q.dim() == 4 and k.dim() == 4 and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3]
-              and q.dtype == k.dtype,
-              "cache_weights: q (batch, rows, heads, head_dim), k (batch, length, kv_heads, head_dim) of one type")
+        T = self._types()
+        dt = q.dtype
+        if q.ndim != 4 or k.ndim != 4 or k.dtype is not dt or dt not in T:
+            raise ValueError("cache_weights: q (batch, rows, heads, head_dim), k (batch, length, kv_heads, head_dim) of "
+                             "one type, f16 or bf16")
         B, R, heads, D = q.shape
-        L, kv = k.shape[1:3]
-        _need(acc.shape == (B, kv, L) and str(acc.dtype) == "torch.float32",
-              "cache_weights: acc is f32 of (batch, kv_heads, length)")
-        _need(lens.shape == (B,) and str(lens.dtype) == "torch.int32" and lens.is_contiguous(),
-              "cache_weights: lens is int32 of (batch,)")
-        _need(lse.shape == (B, R, heads) and str(lse.dtype) == "torch.float32" and lse.is_contiguous(),
-              "cache_weights: lse is f32 of (batch, rows, heads)")
-        self._on("cache_weights", q=q, k=k, lens=lens, lse=lse, acc=acc)
-        a = _lib.DcCacheWeight(q.data_ptr(), k.data_ptr(), lens.data_ptr(), lse.data_ptr(), acc.data_ptr(),
-                               *_strides(q, "q"), *_strides(k, "k"), *_strides(acc, "acc"),
-                               D ** -0.5 if scale is None else scale, decay, B, R, heads, kv, D, L,
-                               1 if causal else 0, _type(q))
-        self._check(self.L.dc_cache_weights_dev(self.h, C.byref(a)), "cache_weights")
+        Bk, L, kv, Dk = k.shape
+        if Bk != B or Dk != D or acc.shape != (B, kv, L) or T.get(acc.dtype) != 0:
+            raise ValueError("cache_weights: acc is f32 of (batch, kv_heads, length), q and k of one batch and head_dim")
+        if not self._flat(lens, (B,), T["i32"]):
+            raise ValueError("cache_weights: lens is int32 of (batch,)")
+        if lse.shape != (B, R, heads) or T.get(lse.dtype) != 0 or not lse.is_contiguous():
+            raise ValueError("cache_weights: lse is f32 of (batch, rows, heads)")
+        sq, sk, sa = q.stride(), k.stride(), acc.stride()
+        if sq[3] != 1 or sk[3] != 1 or (sa[2] != 1 and L > 1):
+            raise ValueError("cache_weights: the last dimension of q, k and acc must be contiguous")
+        a = _lib.CACHE_WEIGHT.pack(*self._ptrs("cache_weights", q, k, lens, lse, acc), *sq[:3], *sk[:3], *sa[:2],
+                                   D ** -0.5 if scale is None else scale, decay, B, R, heads, kv, D, L,
+                                   1 if causal else 0, T[dt])
+        rc = self.L.dc_cache_weights_dev(self.h, a)
+        if rc:
+            self._check(rc, "cache_weights")
 
     def cache_evict_dev(self, k, v, acc, lens, k_out, v_out, acc_out, index, lens_out, *, budget: int,
                         recent: int = 0) -> None:
@@ -354,31 +369,34 @@ class Compute:
         (batch, int32).  What lies behind a sequence's last kept token is left as
         it is.  Heads keep different tokens but equally many.  The outputs must not
         overlap the inputs."""
-        budget, recent = int(budget), int(recent)
-        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
-              "cache_evict: k and v are (batch, length, kv_heads, head_dim) of one type")
+        T = self._types()
+        budget, recent, dt = int(budget), int(recent), k.dtype
+        if k.ndim != 4 or v.shape != k.shape or v.dtype is not dt or dt not in T:
+            raise ValueError("cache_evict: k and v are (batch, length, kv_heads, head_dim) of one type")
         B, L, kv, D = k.shape
         room = min(budget, L)
-        _need(k_out.shape == v_out.shape and k_out.dim() == 4 and k_out.dtype == v_out.dtype == k.dtype
-              and (k_out.shape[0], *k_out.shape[2:]) == (B, kv, D) and k_out.shape[1] >= room,
-              "cache_evict: k_out and v_out are as k, with room for the budget")
-        for name, t, kind in (("acc", acc, "torch.float32"), ("acc_out", acc_out, "torch.float32"),
-                              ("index", index, "torch.int32")):
-            _need(t.dim() == 3 and t.shape[:2] == (B, kv) and str(t.dtype) == kind
-                  and (t.shape[2] == L if name == "acc" else t.shape[2] >= room),
-                  f"cache_evict: {name} is {kind[6:]} of (batch, kv_heads, tokens)")
-        for name, t in (("lens", lens), ("lens_out", lens_out)):
-            _need(t.shape == (B,) and str(t.dtype) == "torch.int32" and t.is_contiguous(),
-                  f"cache_evict: {name} is int32 of (batch,)")
-        self._on("cache_evict", k=k, v=v, acc=acc, lens=lens, k_out=k_out, v_out=v_out, acc_out=acc_out, index=index,
-                 lens_out=lens_out)
-        _type(k)
-        a = _lib.DcCacheEvict(
-            *(t.data_ptr() for t in (k, v, acc, lens, k_out, v_out, acc_out, index, lens_out)),
-            *_strides(k, "k"), *_strides(v, "v"), *_strides(acc, "acc"), *_strides(k_out, "k_out"),
-            *_strides(v_out, "v_out"), *_strides(acc_out, "acc_out"), *_strides(index, "index"),
+        if k_out.ndim != 4 or v_out.shape != k_out.shape or k_out.dtype is not dt or v_out.dtype is not dt or (
+                k_out.shape[1] < room or k_out.shape != (B, k_out.shape[1], kv, D)):
+            raise ValueError("cache_evict: k_out and v_out are as k, with room for the budget")
+        if acc.shape != (B, kv, L) or T.get(acc.dtype) != 0:
+            raise ValueError("cache_evict: acc is f32 of (batch, kv_heads, length)")
+        for t, ok in ((acc_out, T.get(acc_out.dtype) == 0), (index, index.dtype is T["i32"])):
+            if not ok or t.ndim != 3 or t.shape[2] < room or t.shape != (B, kv, t.shape[2]):
+                raise ValueError("cache_evict: acc_out is f32 and index int32 of (batch, kv_heads, room for the budget)")
+        if not (self._flat(lens, (B,), T["i32"]) and self._flat(lens_out, (B,), T["i32"])):
+            raise ValueError("cache_evict: lens and lens_out are int32 of (batch,)")
+        strides = []
+        for t in (k, v, acc, k_out, v_out, acc_out, index):
+            s = t.stride()
+            if s[-1] != 1 and t.shape[-1] > 1:
+                raise ValueError("cache_evict: the last dimension of every buffer must be contiguous")
+            strides += s[:-1]
+        a = _lib.CACHE_EVICT.pack(
+            *self._ptrs("cache_evict", k, v, acc, lens, k_out, v_out, acc_out, index, lens_out), *strides,
             B, kv, D, L, budget, recent, k.element_size())
-        self._check(self.L.dc_cache_evict_dev(self.h, C.byref(a)), "cache_evict")
+        rc = self.L.dc_cache_evict_dev(self.h, a)
+        if rc:
+            self._check(rc, "cache_evict")
 
     def measure_capacity(self, spec=None, T: int = 16, seconds: float = 0.3) -> float:
         """The capacity the ring's planner apportions layers by, in the

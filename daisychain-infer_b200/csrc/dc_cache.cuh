@@ -52,11 +52,12 @@ static inline Span span(const void* p, int elem, std::initializer_list<Dim> dims
   s.hi = s.lo + (uintptr_t)(last + 1) * elem;
   return s;
 }
-// Whether a buffer of es-byte elements begins, and each of its rows (at these
-// strides), on a boundary of `align` bytes.
-static inline bool aligned(const void* p, int es, int align, std::initializer_list<int64_t> strides) {
+// Whether a buffer of es-byte elements begins, and each of its rows in these
+// dimensions, on a boundary of `align` bytes.
+static inline bool aligned(const void* p, int es, int align, std::initializer_list<Dim> dims) {
   uintptr_t m = (uintptr_t)p;
-  for (int64_t s : strides) m |= (uintptr_t)(s * es);
+  for (const Dim& d : dims)
+    if (d.n > 1) m |= (uintptr_t)(d.stride * es);
   return !(m & (align - 1));
 }
 

@@ -249,9 +249,12 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
   const int most = std::min(A.budget, A.cache);  // tokens that may be written
   if (!A.lens || !A.lens_out || (most && (!A.k || !A.v || !A.acc || !A.k_out || !A.v_out || !A.acc_out || !A.index)))
     return dc_fail(ctx, DC_E_INVAL, "cache_evict: null buffer");
-  if (most && (!aligned(A.k, es, 16, {A.k_seq, A.k_tok, A.k_head}) || !aligned(A.v, es, 16, {A.v_seq, A.v_tok, A.v_head}) ||
-               !aligned(A.k_out, es, 16, {A.ko_seq, A.ko_tok, A.ko_head}) ||
-               !aligned(A.v_out, es, 16, {A.vo_seq, A.vo_tok, A.vo_head})))
+  auto row_ok = [&](const void* p, int64_t seq, int64_t n, int64_t tok, int64_t head) {
+    return aligned(p, es, 16, {{A.batch, seq}, {n, tok}, {A.kv_heads, head}});
+  };
+  if (most && (!row_ok(A.k, A.k_seq, A.cache, A.k_tok, A.k_head) || !row_ok(A.v, A.v_seq, A.cache, A.v_tok, A.v_head) ||
+               !row_ok(A.k_out, A.ko_seq, most, A.ko_tok, A.ko_head) ||
+               !row_ok(A.v_out, A.vo_seq, most, A.vo_tok, A.vo_head)))
     return dc_fail(ctx, DC_E_INVAL, "cache_evict: k and v rows must begin on 16-byte boundaries");
   const Span in[4] = {
       span(A.k, es, {{A.batch, A.k_seq}, {A.cache, A.k_tok}, {A.kv_heads, A.k_head}, {A.head_dim, 1}}),

@@ -562,11 +562,15 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
   if (!A.q || !A.out || (A.prefix && (!A.k_pre || !A.v_pre)) || (A.own_max && (!A.k_own || !A.v_own || !A.lens)))
     return dc_fail(ctx, DC_E_INVAL, "prefix_attention: null buffer");
   const int es_o = elem_size(A.out_type);
-  if (!aligned(A.q, 2, 16, {A.q_seq, A.q_row, A.q_head}) ||
-      !aligned(A.out, es_o, 16, {A.out_seq, A.out_row, A.out_head}) ||
-      (A.prefix && (!aligned(A.k_pre, 2, 16, {A.kp_tok, A.kp_head}) || !aligned(A.v_pre, 2, 16, {A.vp_tok, A.vp_head}))) ||
-      (A.own_max && (!aligned(A.k_own, 2, 16, {A.ko_seq, A.ko_tok, A.ko_head}) ||
-                     !aligned(A.v_own, 2, 16, {A.vo_seq, A.vo_tok, A.vo_head}))))
+  auto row_ok = [&](const void* p, int es, int64_t seq, int64_t n, int64_t tok, int heads, int64_t head) {
+    return aligned(p, es, 16, {{A.batch, seq}, {n, tok}, {heads, head}});
+  };
+  if (!row_ok(A.q, 2, A.q_seq, A.rows, A.q_row, A.heads, A.q_head) ||
+      !row_ok(A.out, es_o, A.out_seq, A.rows, A.out_row, A.heads, A.out_head) ||
+      (A.prefix && (!row_ok(A.k_pre, 2, 0, A.prefix, A.kp_tok, A.kv_heads, A.kp_head) ||
+                    !row_ok(A.v_pre, 2, 0, A.prefix, A.vp_tok, A.kv_heads, A.vp_head))) ||
+      (A.own_max && (!row_ok(A.k_own, 2, A.ko_seq, A.own_max, A.ko_tok, A.kv_heads, A.ko_head) ||
+                     !row_ok(A.v_own, 2, A.vo_seq, A.own_max, A.vo_tok, A.kv_heads, A.vo_head))))
     return dc_fail(ctx, DC_E_INVAL, "prefix_attention: q, k, v and out rows must begin on 16-byte boundaries");
   const Plan pl = make_plan(A, ctx->sm_count);
   const size_t need = ws_bytes_of(pl);

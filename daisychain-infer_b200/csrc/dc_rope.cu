@@ -9,8 +9,8 @@
 // Bound by HBM: every element is read once and written once, so nothing is
 // staged.  A head belongs to hd/8 neighbouring lanes; a lane holds four
 // channels i.. and their partners i + rot/2.., so the rotation needs no
-// exchange and the norm one shuffle tree.  The cosines and sines of a row are
-// formed once for all its heads: the angle in turns (position x frequency / 2
+// exchange and the norm one shuffle tree, and a warp walks a row's heads with
+// the lane's angles in registers: the angle in turns (position x frequency / 2
 // pi) in 64 bits, where a position of a million still has 33 bits behind the
 // point, its fraction rounded to f32 for sincospi.
 #include <math.h>
@@ -24,6 +24,9 @@ namespace {
 using namespace dcc;
 
 constexpr int THREADS = 256;
+// heads a lane holds at once (32 or 48 registers of raw channels)
+template <typename T>
+constexpr int MAX_STEPS = sizeof(T) == 4 ? 3 : 4;
 constexpr int MAX_PAIRS = DC_MAX_ROT / 2;
 
 struct RopeArgs {
@@ -34,148 +37,239 @@ struct RopeArgs {
   void *q, *k, *v;
   int64_t ldx, ld_pos, q_row, q_head, k_seq, k_tok, k_head, v_seq, v_tok, v_head, cache_len, n_slots;
   float eps, inv_hd;
-  int rows, heads, kv_heads, hd, rot, tasks, per_block, rows_per_block;
+  int rows, heads, kv_heads, hd, rot, parts, q_parts, steps;
+  int64_t items;
   int* status;
   double turns[MAX_PAIRS];  // frequency of each pair / 2 pi
   uint8_t axis[MAX_PAIRS];
 };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool vec, float (&v)[4]) {
-  alignas(16) T h[4];
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = p[i];
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(h) = *reinterpret_cast<const float4*>(p);
-  } else {
-    *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = to_f32(h[i]);
+// Two f32 in a register pair, and the packed operations on them.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool vec, const float (&v)[4]) {
-  alignas(16) T h[4];
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// G neighbouring channels as they lie in memory (VEC: 16-byte pieces).
+template <typename T, int G>
+struct alignas(16) Some {
+  T v[G];
+};
+template <bool VEC, int G, typename T>
+__device__ __forceinline__ Some<T, G> load(const T* p) {
+  Some<T, G> f;
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) h[i] = from_f32<T>(v[i]);
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = h[i];
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(h);
+    for (int i = 0; i < (int)(G * sizeof(T)) / 16; i++)
+      reinterpret_cast<uint4*>(&f)[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+#pragma unroll
+    for (int i = 0; i < G; i++) f.v[i] = p[i];
+  }
+  return f;
+}
+__device__ __forceinline__ F2 pair(const float* p) { return f2(p[0], p[1]); }
+__device__ __forceinline__ F2 pair(const __half* p) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return f2(f.x, f.y);
+}
+__device__ __forceinline__ F2 pair(const __nv_bfloat16* p) {
+  const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+  return f2(f.x, f.y);
+}
+__device__ __forceinline__ void unpair(float* p, float2 f) { p[0] = f.x, p[1] = f.y; }
+__device__ __forceinline__ void unpair(__half* p, float2 f) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(f); }
+__device__ __forceinline__ void unpair(__nv_bfloat16* p, float2 f) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(f);
+}
+template <bool VEC, int G, typename T>
+__device__ __forceinline__ void store(T* p, const F2 (&x)[G / 2]) {
+  Some<T, G> f;
+#pragma unroll
+  for (int i = 0; i < G / 2; i++) unpair(f.v + 2 * i, split(x[i]));
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)(G * sizeof(T)) / 16; i++)
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&f)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < G; i++) p[i] = f.v[i];
   }
 }
 
-// Blocks along x take rows_per_block rows each, blocks along y per_block of
-// their heads (few rows: a block's worth each, so that the call spreads over
-// the SMs; many rows: all).  LANES: lanes of a head, a power of two >= hd / 8.
-template <typename TI, typename TO, int LANES, bool VEC>
-__global__ void __launch_bounds__(THREADS) k_head_norm_rope(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float2 cs[];  // rows_per_block x rot/2
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row0 = blockIdx.x * a.rows_per_block;
-  const int nrows = min(a.rows_per_block, a.rows - row0);
+// A work item is a share of a row's query heads, or of its key and value heads.
+// Its warp holds SEGS = 32 / LANES heads side by side, `steps` deep, and loads
+// all of them, its angles' positions and its slot before it uses any.  A lane
+// holds G channels and their G partners of a head; its angles and weights are
+// the same for every head of the item (the segments share the making of the
+// angles).  Blocks walk the items; the frequencies lie in shared memory, since
+// lanes that read different kernel parameters wait for each other.
+template <typename TI, typename TO, int LANES, int G, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) k_head_norm_rope(const __grid_constant__ RopeArgs a) {
+  constexpr int SEGS = 32 / LANES, EACH = SEGS >= G ? 1 : G / SEGS;  // angles a lane makes
+  constexpr int STEPS = MAX_STEPS<TI>;
+  __shared__ double turns[MAX_PAIRS];
+  __shared__ int64_t pos_at[MAX_PAIRS];
   const int pairs = a.rot >> 1;
-  for (int i = threadIdx.x; i < nrows * pairs; i += THREADS) {
-    const int r = i / pairs, p = i - r * pairs;
-    const double t = (double)a.pos[a.axis[p] * a.ld_pos + row0 + r] * a.turns[p];
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    cs[i] = make_float2(c, s);
+  for (int i = threadIdx.x; i < pairs; i += THREADS) {
+    turns[i] = a.turns[i];
+    pos_at[i] = a.axis[i] * a.ld_pos;
   }
   __syncthreads();
-  const int sub = threadIdx.x & (LANES - 1);
-  const bool live = sub < (a.hd >> 3);
-  const int nrot = a.rot >> 3;
-  // this lane's two groups of four channels: a rotated group and its partners,
-  // or eight channels that are not rotated
-  const bool turn = sub < nrot;
-  const int c0 = turn ? 4 * sub : a.rot + 8 * (sub - nrot);
-  const int c1 = turn ? c0 + pairs : c0 + 4;
-  const int head0 = blockIdx.y * a.per_block;
-  const int nheads = min(a.per_block, a.tasks - head0);
-  const int total = nrows * nheads;
-  // (whole warps stay in the loop: the norm's shuffles name all lanes)
-  for (int base = (threadIdx.x >> 5) * (32 / LANES); base < total; base += THREADS / LANES) {
-    const int task = base + (threadIdx.x & 31) / LANES;
-    const bool on = live && task < total;
-    const int r = task / nheads, head = head0 + task - r * nheads;
-    const int row = row0 + r;
-    const bool is_v = head >= a.heads + a.kv_heads, is_q = head < a.heads;
-    float lo[4] = {0, 0, 0, 0}, hi[4] = {0, 0, 0, 0};
-    const int d0 = is_v ? 8 * sub : c0, d1 = is_v ? 8 * sub + 4 : c1;
-    if (on) {
-      const TI* src = (const TI*)a.x + (int64_t)row * a.ldx + (int64_t)head * a.hd;
-      load4<TI>(src + d0, VEC, lo);
-      load4<TI>(src + d1, VEC, hi);
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, sub = lane & (LANES - 1), seg = lane / LANES;
+  const int nrot = a.rot / (2 * G);
+  const bool live = sub < a.hd / (2 * G), turn = sub < nrot;
+  // this lane's two groups of channels: a rotated group and its partners, or
+  // two groups that are not rotated
+  const int c0 = turn ? G * sub : a.rot + 2 * G * (sub - nrot);
+  const int c1 = turn ? c0 + pairs : c0 + G;
+  for (int64_t id = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); id < a.items;
+       id += (int64_t)gridDim.x * (THREADS / 32)) {
+    const int row = (int)(id / a.parts), part = (int)(id - (int64_t)row * a.parts);
+    const bool is_q = part < a.q_parts;
+    // heads of the item: from h0 of the queries, or of the keys and then values
+    const int h0 = (is_q ? part : part - a.q_parts) * a.steps * SEGS + seg;
+    const int heads = is_q ? a.heads : 2 * a.kv_heads;
+    const TI* x = (const TI*)a.x + row * a.ldx + (is_q ? 0 : a.heads * a.hd);
+    Some<TI, G> lo[STEPS], hi[STEPS];
+#pragma unroll
+    for (int u = 0; u < STEPS; u++) {
+      const int h = h0 + u * SEGS;
+      if (u < a.steps && live && h < heads) {
+        lo[u] = load<VEC, G>(x + h * a.hd + c0);
+        hi[u] = load<VEC, G>(x + h * a.hd + c1);
+      }
     }
+    int64_t slot = is_q ? 0 : a.slots ? a.slots[row] : row;
     const float* w = is_q ? a.wq : a.wk;
-    float ss = 0.0f;
+    Some<float, G> wl, wh;
+    if (w && live) {
+      wl = load<VEC, G>(w + c0);
+      wh = load<VEC, G>(w + c1);
+    }
+    F2 c[G / 2], s[G / 2], ns[G / 2];
+    {
+      float mc[EACH], ms[EACH];
 #pragma unroll
-    for (int i = 0; i < 4; i++) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
+      for (int i = 0; i < EACH; i++) {
+        mc[i] = 1.0f, ms[i] = 0.0f;
+        const int p = c0 + (seg * EACH + i) % G;
+        if (turn) {
+          const double t = (double)a.pos[pos_at[p] + row] * turns[p];
+          sincospif(2.0f * (float)(t - rint(t)), &ms[i], &mc[i]);
+        }
+      }
+      float ca[G], sa[G];
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-    if (!on) continue;
-    TO* dst;
-    if (is_q) {
-      dst = (TO*)a.q + (int64_t)row * a.q_row + (int64_t)head * a.q_head;
-    } else {
-      const int64_t slot = a.slots ? a.slots[row] : row;
-      if (slot < 0) continue;
+      for (int i = 0; i < G; i++) {
+        ca[i] = SEGS == 1 ? mc[i] : __shfl_sync(~0u, mc[i % EACH], sub + i / EACH * LANES);
+        sa[i] = SEGS == 1 ? ms[i] : __shfl_sync(~0u, ms[i % EACH], sub + i / EACH * LANES);
+      }
+#pragma unroll
+      for (int i = 0; i < G / 2; i++) {
+        c[i] = f2(ca[2 * i], ca[2 * i + 1]);
+        s[i] = f2(sa[2 * i], sa[2 * i + 1]);
+        ns[i] = f2(-sa[2 * i], -sa[2 * i + 1]);
+      }
+    }
+    TO *at = (TO*)a.q + row * a.q_row, *v_at = nullptr;
+    int64_t step = a.q_head;
+    if (!is_q) {
       if (slot >= a.n_slots) {
-        atomicOr(a.status, DC_ST_BOUNDS);
-        continue;
+        if (lane == 0) atomicOr(a.status, DC_ST_BOUNDS);
+        slot = -1;
       }
-      const int64_t seq = a.n_slots == a.cache_len ? 0 : slot / a.cache_len;
-      const int64_t tok = slot - seq * a.cache_len;
-      dst = is_v ? (TO*)a.v + seq * a.v_seq + tok * a.v_tok + (head - a.heads - a.kv_heads) * a.v_head
-                 : (TO*)a.k + seq * a.k_seq + tok * a.k_tok + (head - a.heads) * a.k_head;
+      const int64_t seq = a.n_slots == a.cache_len || slot < 0 ? 0 : slot / a.cache_len, tok = slot - seq * a.cache_len;
+      at = (TO*)a.k + seq * a.k_seq + tok * a.k_tok;
+      v_at = (TO*)a.v + seq * a.v_seq + tok * a.v_tok - a.kv_heads * a.v_head;
+      step = a.k_head;
     }
-    if (!is_v) {
+#pragma unroll
+    for (int u = 0; u < STEPS; u++) {
+      if (u >= a.steps) break;
+      const int h = h0 + u * SEGS;
+      const bool is_v = !is_q && h >= a.kv_heads;
+      F2 x0[G / 2], x1[G / 2];
+#pragma unroll
+      for (int i = 0; i < G / 2; i++) x0[i] = pair(lo[u].v + 2 * i), x1[i] = pair(hi[u].v + 2 * i);
       if (w) {
-        const float inv = __frsqrt_rn(fmaf(ss, a.inv_hd, a.eps));
+        F2 sq = mul2(x0[0], x0[0]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          lo[i] = lo[i] * inv * __ldg(w + d0 + i);
-          hi[i] = hi[i] * inv * __ldg(w + d1 + i);
+        for (int i = 1; i < G / 2; i++) sq = fma2(x0[i], x0[i], sq);
+#pragma unroll
+        for (int i = 0; i < G / 2; i++) sq = fma2(x1[i], x1[i], sq);
+        const float2 both = split(sq);
+        float ss = live ? both.x + both.y : 0.0f;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+        const float inv = rsqrtf(fmaf(ss, a.inv_hd, a.eps));
+        if (!is_v) {
+          const F2 inv2 = f2(inv, inv);
+#pragma unroll
+          for (int i = 0; i < G / 2; i++) {
+            x0[i] = mul2(x0[i], mul2(inv2, pair(wl.v + 2 * i)));
+            x1[i] = mul2(x1[i], mul2(inv2, pair(wh.v + 2 * i)));
+          }
         }
       }
-      if (turn) {
+      if (turn && !is_v) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 t = cs[r * pairs + d0 + i];
-          const float l = lo[i], h = hi[i];
-          lo[i] = l * t.x - h * t.y;
-          hi[i] = h * t.x + l * t.y;
+        for (int i = 0; i < G / 2; i++) {
+          const F2 l = x0[i], r = x1[i];
+          x0[i] = fma2(r, ns[i], mul2(l, c[i]));
+          x1[i] = fma2(l, s[i], mul2(r, c[i]));
         }
+      }
+      if (live && h < heads && slot >= 0) {
+        TO* p = is_v ? v_at + h * a.v_head : at + h * step;
+        store<VEC, G>(p + c0, x0);
+        store<VEC, G>(p + c1, x1);
       }
     }
-    store4<TO>(dst + d0, VEC, lo);
-    store4<TO>(dst + d1, VEC, hi);
   }
 }
 
 using Kernel = void (*)(const RopeArgs);
 
-template <typename TI, typename TO, bool VEC>
-Kernel by_lanes(int lanes) {
-  return lanes == 8    ? k_head_norm_rope<TI, TO, 8, VEC>
-         : lanes == 16 ? k_head_norm_rope<TI, TO, 16, VEC>
-                       : k_head_norm_rope<TI, TO, 32, VEC>;
-}
+// hd <= 64, 128 or 256.  Groups of eight channels where rot and hd are
+// multiples of 16 and rows begin on 16-byte boundaries (a quarter fewer
+// instructions a channel than groups of four), else of four, one by one.
 template <typename TI, typename TO>
-Kernel by_vec(int lanes, bool vec) {
-  return vec ? by_lanes<TI, TO, true>(lanes) : by_lanes<TI, TO, false>(lanes);
+Kernel by_size(int hd, bool wide) {
+  if (wide)
+    return hd <= 64    ? k_head_norm_rope<TI, TO, 4, 8, true>
+           : hd <= 128 ? k_head_norm_rope<TI, TO, 8, 8, true>
+                       : k_head_norm_rope<TI, TO, 16, 8, true>;
+  return hd <= 64    ? k_head_norm_rope<TI, TO, 8, 4, false>
+         : hd <= 128 ? k_head_norm_rope<TI, TO, 16, 4, false>
+                     : k_head_norm_rope<TI, TO, 32, 4, false>;
 }
 template <typename TI>
-Kernel by_out(int out, int lanes, bool vec) {
-  return out == DC_F32   ? by_vec<TI, float>(lanes, vec)
-         : out == DC_F16 ? by_vec<TI, __half>(lanes, vec)
-                         : by_vec<TI, __nv_bfloat16>(lanes, vec);
+Kernel by_out(int out, int hd, bool wide) {
+  return out == DC_F32   ? by_size<TI, float>(hd, wide)
+         : out == DC_F16 ? by_size<TI, __half>(hd, wide)
+                         : by_size<TI, __nv_bfloat16>(hd, wide);
 }
 
 }  // namespace
@@ -218,7 +312,7 @@ extern "C" int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* p) {
   if (!A.x || !A.pos || (A.heads && !A.q) || (A.kv_heads && (!A.k || !A.v)))
     return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: null buffer");
   const int64_t width = (int64_t)(A.heads + 2 * A.kv_heads) * A.head_dim;
-  if (A.ldx < width || (A.axes > 1 && A.ld_pos < A.rows))
+  if ((A.rows > 1 && A.ldx < width) || (A.axes > 1 && A.ld_pos < A.rows))
     return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: ldx %lld is below a row's %lld, or ld_pos below the rows",
                    (long long)A.ldx, (long long)width);
   if (A.kv_heads && (A.cache_seqs < 1 || A.cache_len < 1 || A.cache_seqs > INT64_MAX / A.cache_len ||
@@ -249,23 +343,26 @@ extern "C" int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* p) {
   a.cache_len = A.kv_heads ? A.cache_len : 1, a.n_slots = A.kv_heads ? A.cache_seqs * A.cache_len : 1;
   a.eps = (float)A.eps, a.inv_hd = 1.0f / A.head_dim;
   a.rows = A.rows, a.heads = A.heads, a.kv_heads = A.kv_heads, a.hd = A.head_dim, a.rot = A.rot;
-  a.tasks = A.heads + 2 * A.kv_heads;
   a.status = ctx->d_status;
-  const int lanes = A.head_dim <= 64 ? 8 : A.head_dim <= 128 ? 16 : 32;
-  const int at_once = THREADS / lanes;
-  // rows of a block: as many as its threads form angles for in one step, while
-  // the blocks still cover every SM a few times
-  int rpb = pairs ? std::min(8, std::max(1, THREADS / pairs)) : 8;
-  while (rpb > 1 && A.rows / rpb < 4 * ctx->sm_count) rpb >>= 1;
-  a.rows_per_block = rpb;
-  const int blocks = (int)(((int64_t)A.rows + rpb - 1) / rpb);
-  a.per_block = blocks < 2 * ctx->sm_count ? std::min(a.tasks, at_once) : a.tasks;
-  const bool vec = aligned(A.x, es_i, 4 * es_i, {A.ldx}) &&
-                   (!A.heads || aligned(A.q, es_o, 4 * es_o, {A.q_row, A.q_head})) &&
-                   (!A.kv_heads || (aligned(A.k, es_o, 4 * es_o, {A.k_seq, A.k_tok, A.k_head}) &&
-                                    aligned(A.v, es_o, 4 * es_o, {A.v_seq, A.v_tok, A.v_head})));
-  Kernel kern = A.x_type == DC_F32   ? by_out<float>(A.out_type, lanes, vec)
-                : A.x_type == DC_F16 ? by_out<__half>(A.out_type, lanes, vec)
-                                     : by_out<__nv_bfloat16>(A.out_type, lanes, vec);
-  return launch(ctx, kern, dim3(blocks, (a.tasks + a.per_block - 1) / a.per_block), THREADS, rpb * pairs * 8, 1, a);
+  auto row_ok = [](const void* p, int es, std::initializer_list<Dim> dims) { return aligned(p, es, 16, dims); };
+  const bool wide = !(A.rot % 16) && !(A.head_dim % 16) && row_ok(A.x, es_i, {{A.rows, A.ldx}}) && row_ok(A.wq, 4, {}) &&
+                    row_ok(A.wk, 4, {}) && (!A.heads || row_ok(A.q, es_o, {{A.rows, A.q_row}, {A.heads, A.q_head}})) &&
+                    (!A.kv_heads ||
+                     (row_ok(A.k, es_o, {{A.cache_seqs, A.k_seq}, {A.cache_len, A.k_tok}, {A.kv_heads, A.k_head}}) &&
+                      row_ok(A.v, es_o, {{A.cache_seqs, A.v_seq}, {A.cache_len, A.v_tok}, {A.kv_heads, A.v_head}})));
+  // items of a row: as few as the steps allow (each makes the row's angles
+  // again), but enough for 32 warps an SM when rows are few
+  const int segs = 32 / ((A.head_dim <= 64 ? 8 : A.head_dim <= 128 ? 16 : 32) / (wide ? 2 : 1));
+  const int most = A.x_type == DC_F32 ? MAX_STEPS<float> : MAX_STEPS<__half>;
+  const int q_deep = (A.heads + segs - 1) / segs, kv_deep = (2 * A.kv_heads + segs - 1) / segs;
+  const int64_t want = 32 * (int64_t)ctx->sm_count / A.rows;  // items of a row
+  a.steps = (int)std::min<int64_t>(most, std::max<int64_t>(1, (q_deep + kv_deep) / std::max<int64_t>(1, want)));
+  a.q_parts = (q_deep + a.steps - 1) / a.steps;
+  a.parts = a.q_parts + (kv_deep + a.steps - 1) / a.steps;
+  a.items = (int64_t)A.rows * a.parts;
+  Kernel kern = A.x_type == DC_F32   ? by_out<float>(A.out_type, A.head_dim, wide)
+                : A.x_type == DC_F16 ? by_out<__half>(A.out_type, A.head_dim, wide)
+                                     : by_out<__nv_bfloat16>(A.out_type, A.head_dim, wide);
+  const int64_t blocks = std::min<int64_t>((a.items + THREADS / 32 - 1) / (THREADS / 32), 2 * (int64_t)ctx->sm_count);  // (what is resident)
+  return launch(ctx, kern, dim3((unsigned)blocks), THREADS, 0, 1, a);
 }

@@ -274,7 +274,8 @@ extern "C" int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* p) {
   if (!isfinite((float)A.decay)) return dc_fail(ctx, DC_E_INVAL, "cache_weights: decay %g", A.decay);
   if (!A.batch || !A.cache) return DC_OK;
   if (!A.q || !A.k || !A.lens || !A.lse || !A.acc) return dc_fail(ctx, DC_E_INVAL, "cache_weights: null buffer");
-  if (!aligned(A.q, 2, 16, {A.q_seq, A.q_row, A.q_head}) || !aligned(A.k, 2, 16, {A.k_seq, A.k_tok, A.k_head}))
+  if (!aligned(A.q, 2, 16, {{A.batch, A.q_seq}, {A.rows, A.q_row}, {A.heads, A.q_head}}) ||
+      !aligned(A.k, 2, 16, {{A.batch, A.k_seq}, {A.cache, A.k_tok}, {A.kv_heads, A.k_head}}))
     return dc_fail(ctx, DC_E_INVAL, "cache_weights: q and k rows must begin on 16-byte boundaries");
   const Span acc = span(A.acc, 4, {{A.batch, A.acc_seq}, {A.kv_heads, A.acc_head}, {A.cache, 1}});
   const Span in[4] = {span(A.q, 2, {{A.batch, A.q_seq}, {A.rows, A.q_row}, {A.heads, A.q_head}, {A.head_dim, 1}}),
