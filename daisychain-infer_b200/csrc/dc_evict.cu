@@ -4,19 +4,21 @@
 // otherwise the last `recent` and, of the `old` ones before them, the `need` =
 // budget - recent of largest weight (equal ones: lower index), in their order.
 //
-// One cluster of blocks does a (sequence, head): each block holds a slice of the
-// old weights, mapped to whole numbers of the same order, in shared memory.
-// The need-th largest is found digit by digit (four digits of eight bits, most
-// significant first): the blocks count their slices' digits, read each other's
-// counts through distributed shared memory, and all choose the same digit.  Then
-// each block knows how many kept tokens lie before its slice, places its own,
-// and the cluster copies the kept rows, each block an even share.  So weights
-// are read once, only kept rows are read and written, and it is one launch.
+// k_evict_select: one cluster of blocks does a (sequence, head); each block
+// holds a slice of the old weights in shared memory.  The need-th largest is
+// found digit by digit (four digits of eight bits of the weights as whole
+// numbers of the same order, most significant first): the blocks count their
+// slices' digits, read each other's counts through distributed shared memory,
+// and all choose the same digit.  Then each block knows how many kept tokens
+// lie before its slice and places its own.  Weights are read once.  Counting is
+// by lane: a digit has one counter for each of the 32 lanes, in its own bank,
+// since most weights share their leading bits and would otherwise queue for
+// one counter.
 //
-// Bound by HBM through the kept rows' copies (16-byte pieces, eight in flight a
-// thread); the selection costs a few microseconds.  Counting is by lane: a
-// digit has one counter for each of the 32 lanes, in its own bank, since most
-// weights share their leading bits and would otherwise queue for one counter.
+// k_evict_copy: the kept rows, in blocks of about 32 KB of keys and values, all
+// of a block's loads in flight together.  Bound by HBM: only kept rows are
+// read and written.  Blocks of the heads of one run of places are neighbours,
+// since their rows lie side by side.
 #include <algorithm>
 
 #include "dc_cache.cuh"
@@ -29,6 +31,8 @@ constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int DIGITS = 256;
 constexpr int MAX_CLUSTER = 16;
+constexpr int COPIERS = 256;  // threads of a copying block
+constexpr int EACH = 4;       // 16-byte pieces of keys and of values that each holds
 constexpr int SLICE = 32768;  // weights of a block kept on chip; a longer slice is read from memory each time
 
 struct EvArgs {
@@ -41,7 +45,9 @@ struct EvArgs {
   // (strides of k and v in bytes)
   int64_t k_seq, k_tok, k_head, v_seq, v_tok, v_head, acc_seq, acc_head;
   int64_t ko_seq, ko_tok, ko_head, vo_seq, vo_tok, vo_head, acco_seq, acco_head, idx_seq, idx_head;
-  int kv_heads, pieces, cache, budget, recent, cluster, slice;
+  int kv_heads, cache, budget, recent, cluster, slice;
+  int pieces, rows, runs;  // 16-byte pieces of a row, rows of a copying block, its blocks a head
+  uint32_t inverse;        // ceil(2^32 / pieces)
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -68,13 +74,15 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(THREADS) k_cache_evict(const __grid_constant__ EvArgs a) {
-  extern __shared__ uint32_t keys[];         // the slice's weights as whole numbers
-  __shared__ int lanes[DIGITS * 32];         // counts by digit and lane
+__global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant__ EvArgs a) {
+  extern __shared__ float slice[];           // the block's weights
+  __shared__ __align__(16) int lanes[DIGITS * 32];        // counts by digit and lane
   __shared__ int count[4][DIGITS];           // the block's counts of each pass, for the cluster
+  __shared__ int total[DIGITS];              // the cluster's
   __shared__ int chosen[2];                  // a pass's digit, and what is still to be taken of it
-  __shared__ int warp_gt[WARPS + 1], warp_eq[WARPS + 1];
+  __shared__ int warp_gt[WARPS], warp_eq[WARPS];
   __shared__ int block_n[2];                 // the slice's weights above and equal to the last one kept
+  __shared__ int before_n[2];                // those of the blocks before
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -86,151 +94,181 @@ __global__ void __launch_bounds__(THREADS) k_cache_evict(const __grid_constant__
   int32_t* index = a.index + b * a.idx_seq + h * a.idx_head;
   if (h == 0 && rank == 0 && tid == 0) a.lens_out[b] = kept;
 
-  if (n <= a.budget) {  // (the whole cluster: n is its sequence's)
+  // (whole clusters take one way: n is their sequence's)
+  if (n <= a.budget) {
     for (int i = rank * THREADS + tid; i < n; i += a.cluster * THREADS) {
       index[i] = i;
       acc_out[i] = acc[i];
     }
-  } else {
-    const int old = n - a.recent, need = a.budget - a.recent;  // recent <= budget < n
-    const int lo = min(old, (int)rank * a.slice), size = min(old, lo + a.slice) - lo;
-    const bool on_chip = a.slice <= SLICE;
-    if (on_chip && need > 0) {
-      for (int i = tid; i < size; i += THREADS) keys[i] = ordered(acc[lo + i]);
+    return;
+  }
+  const int old = n - a.recent, need = a.budget - a.recent;  // recent <= budget < n
+  for (int i = rank * THREADS + tid; i < a.recent; i += a.cluster * THREADS) {
+    index[need + i] = old + i;
+    acc_out[need + i] = acc[old + i];
+  }
+  if (need == 0) return;
+  const int lo = min(old, (int)rank * a.slice), size = min(old, lo + a.slice) - lo;
+  const bool on_chip = a.slice <= SLICE;
+  if (on_chip) {
+    // (eight loads in flight a thread)
+    for (int i0 = tid; i0 < size; i0 += 8 * THREADS) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (i0 + j * THREADS < size) x[j] = acc[lo + i0 + j * THREADS];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (i0 + j * THREADS < size) slice[i0 + j * THREADS] = x[j];
     }
-    auto key = [&](int i) { return on_chip ? keys[i] : ordered(acc[lo + i]); };
-    uint32_t top = 0;  // the digits found
-    int left = need;   // to be taken of the weights that share them
-    if (need > 0) {
+  }
+  auto weight = [&](int i) { return on_chip ? slice[i] : acc[lo + i]; };
+  uint32_t top = 0;  // the digits found
+  int left = need;   // to be taken of the weights that share them
 #pragma unroll 1
-      for (int pass = 0; pass < 4; pass++) {
-        const int shift = 24 - 8 * pass;
-        for (int i = tid; i < DIGITS * 32; i += THREADS) lanes[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < size; i += THREADS) {
-          const uint32_t u = key(i);
-          if (pass == 0 || (u >> (shift + 8)) == top) atomicAdd(&lanes[((u >> shift) & 255) * 32 + lane], 1);
-        }
-        __syncthreads();
-        for (int d = warp; d < DIGITS; d += WARPS) {
-          const int c = __reduce_add_sync(~0u, lanes[d * 32 + lane]);
-          if (lane == 0) count[pass][d] = c;
-        }
-        cluster_sync();
-        if (warp == 0) {
-          // lane's digits are 255 - 8 lane and the seven below, the largest first
-          int c[8], s = 0;
-#pragma unroll
-          for (int j = 0; j < 8; j++) c[j] = 0;
-          for (int r = 0; r < a.cluster; r++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) c[j] += peer_int(&count[pass][255 - 8 * lane - j], r);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j++) s += c[j];
-          int before = s;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(~0u, before, o);
-            if (lane >= o) before += x;
-          }
-          before -= s;
-          if (before < left && before + s >= left) {
-            int want = left - before, d = 255 - 8 * lane;
-#pragma unroll
-            for (int j = 0; j < 7; j++)
-              if (255 - 8 * lane - j == d && want > c[j]) {
-                want -= c[j];
-                d--;
-              }
-            chosen[0] = d;
-            chosen[1] = want;
-          }
-        }
-        __syncthreads();
-        top = top << 8 | chosen[0];
-        left = chosen[1];
-      }
+  for (int pass = 0; pass < 4; pass++) {
+    const int shift = 24 - 8 * pass;
+    for (int i = tid; i < DIGITS * 32 / 4; i += THREADS) reinterpret_cast<int4*>(lanes)[i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < size; i += THREADS) {
+      const uint32_t u = ordered(weight(i));
+      if (pass == 0 || (u >> (shift + 8)) == top) atomicAdd(&lanes[((u >> shift) & 255) * 32 + lane], 1);
     }
-    // every kept weight is above `top`, or one of the first `left` equal to it
-    // (need = 0: none).  A warp takes a run of the slice; counts before it:
-    const int run = (size + WARPS * 32 - 1) / (WARPS * 32) * 32;
-    const int r0 = min(size, warp * run), r1 = min(size, r0 + run);
-    if (need > 0) {
-      int gt = 0, eq = 0;
-      for (int i = r0; i < r1; i += 32) {
-        const bool in = i + lane < r1;
-        const uint32_t u = in ? key(i + lane) : 0;
-        gt += __popc(__ballot_sync(~0u, in && u > top));
-        eq += __popc(__ballot_sync(~0u, in && u == top));
-      }
-      if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
-      __syncthreads();
-      if (tid == 0) {
-        int g = 0, e = 0;
-        for (int w = 0; w < WARPS; w++) {
-          const int x = warp_gt[w], y = warp_eq[w];
-          warp_gt[w] = g, warp_eq[w] = e;
-          g += x, e += y;
-        }
-        block_n[0] = g, block_n[1] = e;
-      }
+    __syncthreads();
+#pragma unroll 4
+    for (int d = warp; d < DIGITS; d += WARPS) {
+      const int c = __reduce_add_sync(~0u, lanes[d * 32 + lane]);
+      if (lane == 0) count[pass][d] = c;
+    }
+    if (a.cluster > 1)
       cluster_sync();
-      int g = warp_gt[warp], e = warp_eq[warp];
-      for (int r = 0; r < (int)rank; r++) g += peer_int(&block_n[0], r), e += peer_int(&block_n[1], r);
-      const unsigned below = (1u << lane) - 1;
-      for (int i = r0; i < r1; i += 32) {
-        const bool in = i + lane < r1;
-        const uint32_t u = in ? key(i + lane) : 0;
-        const unsigned mg = __ballot_sync(~0u, in && u > top), me = __ballot_sync(~0u, in && u == top);
-        const int eb = e + __popc(me & below);
-        if (in && (u > top || (u == top && eb < left))) {
-          const int at = g + __popc(mg & below) + min(eb, left), token = lo + i + lane;
-          index[at] = token;
-          acc_out[at] = acc[token];
-        }
-        g += __popc(mg);
-        e += __popc(me);
+    else
+      __syncthreads();
+    if (tid < DIGITS) {
+      int c = 0;
+#pragma unroll 4
+      for (int r = 0; r < a.cluster; r++) c += peer_int(&count[pass][tid], (rank + r) % a.cluster);
+      total[tid] = c;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // lane's digits are 255 - 8 lane and the seven below, the largest first
+      int c[8], s = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) s += c[j] = total[255 - 8 * lane - j];
+      int before = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(~0u, before, o);
+        if (lane >= o) before += x;
+      }
+      before -= s;
+      if (before < left && before + s >= left) {
+        int want = left - before, d = 255 - 8 * lane;
+#pragma unroll
+        for (int j = 0; j < 7; j++)
+          if (255 - 8 * lane - j == d && want > c[j]) {
+            want -= c[j];
+            d--;
+          }
+        chosen[0] = d;
+        chosen[1] = want;
       }
     }
-    for (int i = rank * THREADS + tid; i < a.recent; i += a.cluster * THREADS) {
-      index[need + i] = old + i;
-      acc_out[need + i] = acc[old + i];
-    }
+    __syncthreads();
+    top = top << 8 | chosen[0];
+    left = chosen[1];
   }
-  cluster_sync();  // the index is complete, and no block reads another's counts any more
+  // every kept weight is above `top`, or one of the first `left` equal to it.
+  // A warp takes a run of the slice; counts before it:
+  const int run = (size + WARPS * 32 - 1) / (WARPS * 32) * 32;
+  const int r0 = min(size, warp * run), r1 = min(size, r0 + run);
+  int gt = 0, eq = 0;
+#pragma unroll 4
+  for (int i = r0; i < r1; i += 32) {
+    const bool in = i + lane < r1;
+    const uint32_t u = in ? ordered(weight(i + lane)) : 0;
+    gt += __popc(__ballot_sync(~0u, in && u > top));
+    eq += __popc(__ballot_sync(~0u, in && u == top));
+  }
+  if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
+  __syncthreads();
+  if (tid == 0) {
+    int g = 0, e = 0;
+    for (int w = 0; w < WARPS; w++) {
+      const int x = warp_gt[w], y = warp_eq[w];
+      warp_gt[w] = g, warp_eq[w] = e;
+      g += x, e += y;
+    }
+    block_n[0] = g, block_n[1] = e;
+    before_n[0] = before_n[1] = 0;
+  }
+  if (a.cluster > 1) {
+    cluster_sync();
+    if (warp == 0) {
+      const bool peer = lane < (int)rank;
+      const int g = __reduce_add_sync(~0u, peer ? peer_int(&block_n[0], lane) : 0);
+      const int e = __reduce_add_sync(~0u, peer ? peer_int(&block_n[1], lane) : 0);
+      if (lane == 0) before_n[0] = g, before_n[1] = e;
+    }
+    cluster_sync();  // (and no block reads another's counts any more: it may end)
+  } else {
+    __syncthreads();
+  }
+  int g = before_n[0] + warp_gt[warp], e = before_n[1] + warp_eq[warp];
+  const unsigned below = (1u << lane) - 1;
+  for (int i = r0; i < r1; i += 32) {
+    const bool in = i + lane < r1;
+    const float w = in ? weight(i + lane) : 0.0f;
+    const uint32_t u = ordered(w);
+    const unsigned mg = __ballot_sync(~0u, in && u > top), me = __ballot_sync(~0u, in && u == top);
+    const int eb = e + __popc(me & below);
+    if (in && (u > top || (u == top && eb < left))) {
+      const int at = g + __popc(mg & below) + min(eb, left);
+      index[at] = lo + i + lane;
+      acc_out[at] = w;
+    }
+    g += __popc(mg);
+    e += __popc(me);
+  }
+}
 
-  // the kept rows: a thread copies one 16-byte piece of a key and of a value row
-  // at a time, four rows in flight
-  const int per = THREADS / a.pieces;  // rows of a step
-  const int r = tid / a.pieces;
-  const int64_t piece = (int64_t)(tid - r * a.pieces) * 16;
-  if (r >= per) return;
-  const uint8_t* k = a.k + b * a.k_seq + h * a.k_head + piece;
-  const uint8_t* v = a.v + b * a.v_seq + h * a.v_head + piece;
-  uint8_t* ko = a.k_out + b * a.ko_seq + h * a.ko_head + piece;
-  uint8_t* vo = a.v_out + b * a.vo_seq + h * a.vo_head + piece;
-  const int step = per * a.cluster;
-  for (int i0 = rank * per + r; i0 < kept; i0 += 4 * step) {
-    uint4 x[4], y[4];
+__global__ void __launch_bounds__(COPIERS, 4) k_evict_copy(const __grid_constant__ EvArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int id = blockIdx.x;
+  const int h = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int run = id % a.runs, b = id / a.runs;
+  const int kept = min(max(0, min(a.lens[b], a.cache)), a.budget);
+  const int i0 = run * a.rows, pieces = min(a.rows, kept - i0) * a.pieces;
+  if (pieces <= 0) return;
+  const int32_t* index = a.index + b * a.idx_seq + h * a.idx_head + i0;
+  const uint8_t *k = a.k + b * a.k_seq + h * a.k_head, *v = a.v + b * a.v_seq + h * a.v_head;
+  uint8_t *ko = a.k_out + b * a.ko_seq + h * a.ko_head, *vo = a.v_out + b * a.vo_seq + h * a.vo_head;
+  uint4 x[EACH], y[EACH];
+  int row[EACH], off[EACH];
+  int64_t token[EACH];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int i = i0 + j * step;
-      if (i < kept) {
-        const int64_t token = __ldcg(index + i);
-        x[j] = *reinterpret_cast<const uint4*>(k + token * a.k_tok);
-        y[j] = *reinterpret_cast<const uint4*>(v + token * a.v_tok);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int64_t i = i0 + j * step;
-      if (i < kept) {
-        *reinterpret_cast<uint4*>(ko + i * a.ko_tok) = x[j];
-        *reinterpret_cast<uint4*>(vo + i * a.vo_tok) = y[j];
-      }
-    }
+  for (int j = 0; j < EACH; j++) {
+    const int p = j * COPIERS + threadIdx.x;
+    row[j] = a.pieces == 1 ? p : __umulhi(p, a.inverse);  // p / pieces: exact for p < 2^16
+    off[j] = (p - row[j] * a.pieces) * 16;
+    token[j] = p < pieces ? index[row[j]] : -1;
   }
+#pragma unroll
+  for (int j = 0; j < EACH; j++)
+    if (token[j] >= 0) {
+      x[j] = *reinterpret_cast<const uint4*>(k + token[j] * a.k_tok + off[j]);
+      y[j] = *reinterpret_cast<const uint4*>(v + token[j] * a.v_tok + off[j]);
+    }
+#pragma unroll
+  for (int j = 0; j < EACH; j++)
+    if (token[j] >= 0) {
+      *reinterpret_cast<uint4*>(ko + (int64_t)(i0 + row[j]) * a.ko_tok + off[j]) = x[j];
+      *reinterpret_cast<uint4*>(vo + (int64_t)(i0 + row[j]) * a.vo_tok + off[j]) = y[j];
+    }
 }
 
 }  // namespace
@@ -243,7 +281,7 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
   if (A.budget < 0 || A.recent < 0 || A.recent > A.budget)
     return dc_fail(ctx, DC_E_INVAL, "cache_evict: recent %d, budget %d", A.recent, A.budget);
   const int es = A.elem_bytes;
-  if ((es != 2 && es != 4) || A.head_dim < 1 || (int64_t)A.head_dim * es % 16 || A.head_dim > THREADS * 16 / es)
+  if ((es != 2 && es != 4) || A.head_dim < 1 || (int64_t)A.head_dim * es % 16 || A.head_dim > COPIERS * EACH * 16 / es)
     return dc_fail(ctx, DC_E_INVAL, "cache_evict: rows of %d elements of %d bytes", A.head_dim, es);
   if (!A.batch) return DC_OK;
   const int most = std::min(A.budget, A.cache);  // tokens that may be written
@@ -287,8 +325,11 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
   a.vo_seq = A.vo_seq * es, a.vo_tok = A.vo_tok * es, a.vo_head = A.vo_head * es;
   a.acc_seq = A.acc_seq, a.acc_head = A.acc_head, a.acco_seq = A.acco_seq, a.acco_head = A.acco_head;
   a.idx_seq = A.idx_seq, a.idx_head = A.idx_head;
-  a.kv_heads = A.kv_heads, a.pieces = A.head_dim * es / 16, a.cache = A.cache;
-  a.budget = A.budget, a.recent = A.recent;
+  a.kv_heads = A.kv_heads, a.cache = A.cache, a.budget = A.budget, a.recent = A.recent;
+  a.pieces = A.head_dim * es / 16;
+  a.inverse = (uint32_t)(((1ull << 32) + a.pieces - 1) / a.pieces);
+  a.rows = COPIERS * EACH / a.pieces;
+  a.runs = (most + a.rows - 1) / a.rows;
   // blocks of a head: until the call fills every SM, but no fewer than 128
   // tokens a block
   const int64_t heads = (int64_t)A.batch * A.kv_heads;
@@ -296,8 +337,10 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
   while (cl < MAX_CLUSTER && heads * cl < ctx->sm_count && A.cache >= 256 * cl) cl <<= 1;
   a.cluster = cl;
   a.slice = (std::max(1, A.cache) + cl - 1) / cl;
+  if (heads * std::max(a.runs, cl) > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "cache_evict: too many blocks");
   if (cl > 8)
-    DC_CUDA(ctx, cudaFuncSetAttribute((const void*)k_cache_evict, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  const int smem = a.slice <= SLICE ? a.slice * 4 : 0;
-  return launch(ctx, k_cache_evict, dim3((unsigned)(heads * cl)), THREADS, smem, cl, a);
+    DC_CUDA(ctx, cudaFuncSetAttribute((const void*)k_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (int rc = launch(ctx, k_evict_select, dim3((unsigned)(heads * cl)), THREADS, a.slice <= SLICE ? a.slice * 4 : 0, cl, a))
+    return rc;
+  return most ? launch(ctx, k_evict_copy, dim3((unsigned)(heads * a.runs)), COPIERS, 0, 1, a) : DC_OK;
 }
