@@ -5,15 +5,15 @@
 // budget - recent of largest weight (equal ones: lower index), in their order.
 //
 // k_evict_select: one cluster of blocks does a (sequence, head); each block
-// holds a slice of the old weights in shared memory.  The need-th largest is
-// found digit by digit (four digits of eight bits of the weights as whole
-// numbers of the same order, most significant first): the blocks count their
-// slices' digits, read each other's counts through distributed shared memory,
-// and all choose the same digit.  Then each block knows how many kept tokens
-// lie before its slice and places its own.  Weights are read once.  Counting is
-// by lane: a digit has one counter for each of the 32 lanes, in its own bank,
-// since most weights share their leading bits and would otherwise queue for
-// one counter.
+// holds a slice of the old weights, mapped to whole numbers of the same order,
+// in shared memory.  The need-th largest is found digit by digit (four digits
+// of eight bits, most significant first): the blocks count their slices'
+// digits, add the counts to each other's totals through distributed shared
+// memory, and all choose the same digit.  Then each block knows how many kept tokens lie before
+// its slice and places its own.  Weights are read once.  Counting goes to eight
+// copies of the counters, since most weights share their leading bits and
+// would otherwise queue for one.  What bounds it is latency: barriers, and the
+// first fetch of each instruction, which is why its loops are not unrolled.
 //
 // k_evict_copy: the kept rows, in blocks of about 32 KB of keys and values, all
 // of a block's loads in flight together.  Bound by HBM: only kept rows are
@@ -33,7 +33,8 @@ constexpr int DIGITS = 256;
 constexpr int MAX_CLUSTER = 16;
 constexpr int COPIERS = 256;  // threads of a copying block
 constexpr int EACH = 4;       // 16-byte pieces of keys and of values that each holds
-constexpr int SLICE = 32768;  // weights of a block kept on chip; a longer slice is read from memory each time
+constexpr int SLICE = 16384;  // weights of a block kept on chip; those of a longer slice are read each time
+constexpr int COPIES = 8;     // of the counters
 
 struct EvArgs {
   const uint8_t *k, *v;
@@ -66,6 +67,12 @@ __device__ __forceinline__ int peer_int(const int* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
+// Adds v to the int at shared address p of block `rank`.
+__device__ __forceinline__ void peer_add(const int* p, uint32_t rank, int v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(dcp::smem_u32(p)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
 // Whole numbers in the order of the floats: NaN below -inf, -0 equal to 0.
 __device__ __forceinline__ uint32_t ordered(float f) {
   uint32_t u = __float_as_uint(f);
@@ -75,14 +82,11 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 
 __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant__ EvArgs a) {
-  extern __shared__ float slice[];           // the block's weights
-  __shared__ __align__(16) int lanes[DIGITS * 32];        // counts by digit and lane
-  __shared__ int count[4][DIGITS];           // the block's counts of each pass, for the cluster
-  __shared__ int total[DIGITS];              // the cluster's
-  __shared__ int chosen[2];                  // a pass's digit, and what is still to be taken of it
+  extern __shared__ uint32_t slice[];  // the block's weights
+  __shared__ __align__(16) int counters[COPIES * DIGITS];
+  __shared__ __align__(16) int totals[4][DIGITS];  // the cluster's counts of each pass
   __shared__ int warp_gt[WARPS], warp_eq[WARPS];
-  __shared__ int block_n[2];                 // the slice's weights above and equal to the last one kept
-  __shared__ int before_n[2];                // those of the blocks before
+  __shared__ int block_n[2];        // the slice's weights above and equal to the last one kept
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -110,128 +114,125 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
   if (need == 0) return;
   const int lo = min(old, (int)rank * a.slice), size = min(old, lo + a.slice) - lo;
   const bool on_chip = a.slice <= SLICE;
+  if (tid < DIGITS) reinterpret_cast<int4*>(totals)[tid] = make_int4(0, 0, 0, 0);
+  if (a.cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for below)
   if (on_chip) {
-    // (eight loads in flight a thread)
-    for (int i0 = tid; i0 < size; i0 += 8 * THREADS) {
-      float x[8];
+#pragma unroll 1
+    for (int i0 = tid; i0 < size; i0 += 4 * THREADS) {
+      float x[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (i0 + j * THREADS < size) x[j] = acc[lo + i0 + j * THREADS];
+      for (int j = 0; j < 4; j++) x[j] = i0 + j * THREADS < size ? acc[lo + i0 + j * THREADS] : 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (i0 + j * THREADS < size) slice[i0 + j * THREADS] = x[j];
+      for (int j = 0; j < 4; j++)
+        if (i0 + j * THREADS < size) slice[i0 + j * THREADS] = ordered(x[j]);
     }
   }
-  auto weight = [&](int i) { return on_chip ? slice[i] : acc[lo + i]; };
+  auto weight = [&](int i) { return on_chip ? slice[i] : ordered(__ldg(acc + lo + i)); };
   uint32_t top = 0;  // the digits found
   int left = need;   // to be taken of the weights that share them
 #pragma unroll 1
   for (int pass = 0; pass < 4; pass++) {
     const int shift = 24 - 8 * pass;
-    for (int i = tid; i < DIGITS * 32 / 4; i += THREADS) reinterpret_cast<int4*>(lanes)[i] = make_int4(0, 0, 0, 0);
+    reinterpret_cast<int4*>(counters)[tid] = make_int4(0, 0, 0, 0);
     __syncthreads();
-#pragma unroll 4
-    for (int i = tid; i < size; i += THREADS) {
-      const uint32_t u = ordered(weight(i));
-      if (pass == 0 || (u >> (shift + 8)) == top) atomicAdd(&lanes[((u >> shift) & 255) * 32 + lane], 1);
+    int* mine = counters + (lane & (COPIES - 1)) * DIGITS;
+#pragma unroll 1
+    for (int i0 = tid; i0 < size; i0 += 4 * THREADS) {
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) u[j] = i0 + j * THREADS < size ? weight(i0 + j * THREADS) : 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i0 + j * THREADS < size && (pass == 0 || (u[j] >> (shift + 8)) == top))
+          atomicAdd(mine + ((u[j] >> shift) & 255), 1);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int d = warp; d < DIGITS; d += WARPS) {
-      const int c = __reduce_add_sync(~0u, lanes[d * 32 + lane]);
-      if (lane == 0) count[pass][d] = c;
+    int* total = totals[pass];
+    if (a.cluster > 1 && pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid < DIGITS) {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < COPIES; j++) c += counters[j * DIGITS + tid];
+      // (a few digits hold all the weights: most lanes have nothing to add)
+      if (a.cluster == 1)
+        total[tid] = c;
+      else if (c)
+        for (int r = 0; r < a.cluster; r++) peer_add(&total[tid], (rank + r) & (a.cluster - 1), c);
     }
     if (a.cluster > 1)
       cluster_sync();
     else
       __syncthreads();
-    if (tid < DIGITS) {
-      int c = 0;
-#pragma unroll 4
-      for (int r = 0; r < a.cluster; r++) c += peer_int(&count[pass][tid], (rank + r) % a.cluster);
-      total[tid] = c;
+    // every warp finds the digit: lane's are 255 - 8 lane and the seven below,
+    // the largest first
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum += total[255 - 8 * lane - j];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, before, o);
+      if (lane >= o) before += x;
     }
-    __syncthreads();
-    if (warp == 0) {
-      // lane's digits are 255 - 8 lane and the seven below, the largest first
-      int c[8], s = 0;
+    before -= sum;
+    const int owner = __ffs(__ballot_sync(~0u, before < left && before + sum >= left)) - 1;
+    left -= __shfl_sync(~0u, before, owner);
+    // of the owner's eight digits (lanes 0 to 7 look at one each)
+    const int c8 = lane < 8 ? total[255 - 8 * owner - lane] : 0;
+    int upto = c8;
 #pragma unroll
-      for (int j = 0; j < 8; j++) s += c[j] = total[255 - 8 * lane - j];
-      int before = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(~0u, before, o);
-        if (lane >= o) before += x;
-      }
-      before -= s;
-      if (before < left && before + s >= left) {
-        int want = left - before, d = 255 - 8 * lane;
-#pragma unroll
-        for (int j = 0; j < 7; j++)
-          if (255 - 8 * lane - j == d && want > c[j]) {
-            want -= c[j];
-            d--;
-          }
-        chosen[0] = d;
-        chosen[1] = want;
-      }
+    for (int o = 1; o < 8; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += x;
     }
-    __syncthreads();
-    top = top << 8 | chosen[0];
-    left = chosen[1];
+    const int at = __ffs(__ballot_sync(~0u, lane < 8 && upto >= left)) - 1;
+    left -= __shfl_sync(~0u, upto - c8, at);
+    top = top << 8 | (255 - 8 * owner - at);
   }
   // every kept weight is above `top`, or one of the first `left` equal to it.
-  // A warp takes a run of the slice; counts before it:
+  // A warp takes a run of the slice; counts of both before it:
   const int run = (size + WARPS * 32 - 1) / (WARPS * 32) * 32;
   const int r0 = min(size, warp * run), r1 = min(size, r0 + run);
   int gt = 0, eq = 0;
-#pragma unroll 4
-  for (int i = r0; i < r1; i += 32) {
-    const bool in = i + lane < r1;
-    const uint32_t u = in ? ordered(weight(i + lane)) : 0;
-    gt += __popc(__ballot_sync(~0u, in && u > top));
-    eq += __popc(__ballot_sync(~0u, in && u == top));
+#pragma unroll 2
+  for (int i = r0 + lane; i - lane < r1; i += 32) {
+    const uint32_t u = i < r1 ? weight(i) : 0;
+    gt += i < r1 && u > top;
+    eq += i < r1 && u == top;
   }
+  gt = __reduce_add_sync(~0u, gt), eq = __reduce_add_sync(~0u, eq);
   if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
   __syncthreads();
-  if (tid == 0) {
-    int g = 0, e = 0;
-    for (int w = 0; w < WARPS; w++) {
-      const int x = warp_gt[w], y = warp_eq[w];
-      warp_gt[w] = g, warp_eq[w] = e;
-      g += x, e += y;
-    }
-    block_n[0] = g, block_n[1] = e;
-    before_n[0] = before_n[1] = 0;
-  }
+  const int wg = lane < WARPS ? warp_gt[lane] : 0, we = lane < WARPS ? warp_eq[lane] : 0;
+  int g = __reduce_add_sync(~0u, lane < warp ? wg : 0), e = __reduce_add_sync(~0u, lane < warp ? we : 0);
   if (a.cluster > 1) {
-    cluster_sync();
     if (warp == 0) {
-      const bool peer = lane < (int)rank;
-      const int g = __reduce_add_sync(~0u, peer ? peer_int(&block_n[0], lane) : 0);
-      const int e = __reduce_add_sync(~0u, peer ? peer_int(&block_n[1], lane) : 0);
-      if (lane == 0) before_n[0] = g, before_n[1] = e;
+      const int x = __reduce_add_sync(~0u, wg), y = __reduce_add_sync(~0u, we);
+      if (lane == 0) block_n[0] = x, block_n[1] = y;
     }
-    cluster_sync();  // (and no block reads another's counts any more: it may end)
-  } else {
-    __syncthreads();
+    cluster_sync();
+    const bool peer = lane < (int)rank;
+    g += __reduce_add_sync(~0u, peer ? peer_int(&block_n[0], lane) : 0);
+    e += __reduce_add_sync(~0u, peer ? peer_int(&block_n[1], lane) : 0);
+    // (no block ends before the others have read its counts: waited for below)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
-  int g = before_n[0] + warp_gt[warp], e = before_n[1] + warp_eq[warp];
   const unsigned below = (1u << lane) - 1;
-  for (int i = r0; i < r1; i += 32) {
-    const bool in = i + lane < r1;
-    const float w = in ? weight(i + lane) : 0.0f;
-    const uint32_t u = ordered(w);
+#pragma unroll 2
+  for (int i = r0 + lane; i - lane < r1; i += 32) {
+    const bool in = i < r1;
+    const uint32_t u = in ? weight(i) : 0;
     const unsigned mg = __ballot_sync(~0u, in && u > top), me = __ballot_sync(~0u, in && u == top);
     const int eb = e + __popc(me & below);
     if (in && (u > top || (u == top && eb < left))) {
       const int at = g + __popc(mg & below) + min(eb, left);
-      index[at] = lo + i + lane;
-      acc_out[at] = w;
+      index[at] = lo + i;
+      acc_out[at] = __ldg(acc + lo + i);
     }
     g += __popc(mg);
     e += __popc(me);
   }
+  if (a.cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(COPIERS, 4) k_evict_copy(const __grid_constant__ EvArgs a) {
@@ -330,11 +331,12 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
   a.inverse = (uint32_t)(((1ull << 32) + a.pieces - 1) / a.pieces);
   a.rows = COPIERS * EACH / a.pieces;
   a.runs = (most + a.rows - 1) / a.rows;
-  // blocks of a head: until the call fills every SM, but no fewer than 128
-  // tokens a block
+  // blocks of a head: one for each 4096 tokens while the call does not fill
+  // every SM (16 sequences x 8 heads of 16384 tokens: 35 us in clusters of two,
+  // 41 in fours, 63 in eights), and enough to hold the weights on chip
   const int64_t heads = (int64_t)A.batch * A.kv_heads;
   int cl = 1;
-  while (cl < MAX_CLUSTER && heads * cl < ctx->sm_count && A.cache >= 256 * cl) cl <<= 1;
+  while (cl < MAX_CLUSTER && ((heads * cl < ctx->sm_count && A.cache > 4096 * cl) || A.cache > SLICE * cl)) cl <<= 1;
   a.cluster = cl;
   a.slice = (std::max(1, A.cache) + cl - 1) / cl;
   if (heads * std::max(a.runs, cl) > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "cache_evict: too many blocks");
