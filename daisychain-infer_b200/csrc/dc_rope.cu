@@ -18,10 +18,16 @@
 #include <algorithm>
 
 #include "dc_cache.cuh"
+#include "dc_umma.cuh"
 
 namespace {
 
 using namespace dcc;
+using dcu::F2;
+using dcu::f2;
+using dcu::fma2;
+using dcu::mul2;
+using dcu::split;
 
 constexpr int THREADS = 256;
 // heads a lane holds at once (32 or 48 registers of raw channels)
@@ -43,31 +49,6 @@ struct RopeArgs {
   double turns[MAX_PAIRS];  // frequency of each pair / 2 pi
   uint8_t axis[MAX_PAIRS];
 };
-
-// Two f32 in a register pair, and the packed operations on them.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 split(F2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 
 // G neighbouring channels as they lie in memory (VEC: 16-byte pieces).
 template <typename T, int G>

@@ -26,6 +26,7 @@
 namespace {
 
 using namespace dcc;
+using dcu::F2;
 
 constexpr int KEYS = 128;   // keys of a tile: the MMA's M
 constexpr int COLS = 128;   // query rows of a tile: its N
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* kept = smem;
   uint8_t* ring = smem + NP * PANEL_BYTES;
-  float* scales = (float*)(ring + STAGES * PANEL_BYTES);  // lse * log2 e of a tile's columns; +inf where nothing is added
+  float* scales = (float*)(ring + STAGES * PANEL_BYTES);  // -lse * log2 e of a tile's columns; -inf where nothing is added
   uint64_t* full = (uint64_t*)(scales + C::SCALES * COLS);
   uint64_t* empty = full + STAGES;
   uint64_t* s_full = empty + STAGES;  // [2] scores of a buffer are in TMEM
@@ -179,10 +180,10 @@ __global__ void __launch_bounds__(THREADS, 2)
     // column `threadIdx.x` of Q tile t
     auto column = [&](int t) {
       const int col = threadIdx.x, row = t * a.tile_rows + col / a.group;
-      float v = INFINITY;
+      float v = -INFINITY;
       if (col < a.tile_cols && row < a.rows) {
-        v = a.lse[lse_at + (int64_t)row * a.heads + col % a.group] * LOG2E;
-        if (v == -INFINITY) v = INFINITY;
+        v = -a.lse[lse_at + (int64_t)row * a.heads + col % a.group] * LOG2E;
+        if (v == INFINITY) v = -INFINITY;
       }
       return v;
     };
@@ -207,31 +208,41 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int cols = min(a.tile_cols, (a.rows - first_row) * a.group);
       const bool late = __any_sync(~0u, from > 0);
       if (KEEP_Q) sum = 0.0f;
-      float s4[4] = {0, 0, 0, 0};
-#pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 32) {
-        uint32_t s[32];
-        dcu::ld32(lane_at + (i & 1) * COLS + c0, s);
-        dcu::wait_ld(s);
-        const bool masked = late || c0 + 32 > cols;
+      const F2 c2 = dcu::f2(a.c, a.c);
+      F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
+      uint32_t s[2][32];
+      // columns c0 .. c0 + 31, and the next ones' load meanwhile
+      auto add = [&](uint32_t (&x)[32], uint32_t (&next)[32], int c0) {
+        dcu::wait_ld(x);
+        if (c0 + 32 < cols) dcu::ld32(lane_at + (i & 1) * COLS + c0 + 32, next);
         const float4* l4 = reinterpret_cast<const float4*>(L + c0);
+        if (late || c0 + 32 > cols) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            const float e = dcu::ex2(fmaf(__uint_as_float(x[j]), a.c, L[c0 + j]));
+            part[j & 3] = dcu::add2(part[j & 3], dcu::f2(c0 + j < from || c0 + j >= cols ? 0.0f : e, 0.0f));
+          }
+          return;
+        }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const float4 l = l4[j];
-          float e[4] = {dcu::ex2(fmaf(__uint_as_float(s[4 * j]), a.c, -l.x)),
-                        dcu::ex2(fmaf(__uint_as_float(s[4 * j + 1]), a.c, -l.y)),
-                        dcu::ex2(fmaf(__uint_as_float(s[4 * j + 2]), a.c, -l.z)),
-                        dcu::ex2(fmaf(__uint_as_float(s[4 * j + 3]), a.c, -l.w))};
-          if (masked) {
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-              if (c0 + 4 * j + x < from || c0 + 4 * j + x >= cols) e[x] = 0.0f;
-          }
-#pragma unroll
-          for (int x = 0; x < 4; x++) s4[x] += e[x];
+          const float2 t0 = dcu::split(
+              dcu::fma2(dcu::f2(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), c2, dcu::f2(l.x, l.y)));
+          const float2 t1 = dcu::split(
+              dcu::fma2(dcu::f2(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), c2, dcu::f2(l.z, l.w)));
+          part[(2 * j) & 3] = dcu::add2(part[(2 * j) & 3], dcu::f2(dcu::ex2(t0.x), dcu::ex2(t0.y)));
+          part[(2 * j + 1) & 3] = dcu::add2(part[(2 * j + 1) & 3], dcu::f2(dcu::ex2(t1.x), dcu::ex2(t1.y)));
         }
+      };
+      dcu::ld32(lane_at + (i & 1) * COLS, s[0]);
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 64) {
+        add(s[0], s[1], c0);
+        if (c0 + 32 < cols) add(s[1], s[0], c0 + 32);
       }
-      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      const float2 got = dcu::split(dcu::add2(dcu::add2(part[0], part[1]), dcu::add2(part[2], part[3])));
+      sum += got.x + got.y;
       dcu::fence_before();
       __syncwarp();
       if (lane == 0) dcp::mbar_arrive(&s_free[i & 1]);
