@@ -4,33 +4,30 @@
 //
 // over the prefix's tokens and the row's own.  The sum splits by keys: a part
 // with maximum m and sums l = sum 2^(c x - m), o = sum 2^(c x - m) v (c = log2 e)
-// joins another after both are scaled to the larger maximum.  So every block
-// takes one key/value head, one range of keys and up to 128 query rows:
-//   * prefix blocks: rows are (sequence, row, head of the group) -- all rows of
-//     the batch against one reading of the prefix's keys and values;
-//   * own blocks: rows are (row, head of the group) of one sequence.
-// k_prefix_attn writes each block's (m, l, o); k_prefix_join joins them.
+// joins another after both are scaled to the larger maximum.  Three kernels:
+//   * k_shared: the rows of all sequences that use one key/value head, 128 or 256
+//     a block, against a range of the prefix: one reading of its keys and values
+//     for the whole batch;
+//   * k_own: a sequence's rows that use one head against a range of its own keys;
+//   * k_join: the parts of a row, and its last tokens (below).
 //
-// Bound: HBM while a key/value head has up to ~128 rows (a 64-key tile is 32 KB
-// at 43 GB/s an SM, 0.75 us, against 0.3 us of products and as much of
-// exponentials); the exponential unit and the tensor pipe above that.
+// A running maximum is raised only when a row's has grown by more than 2^8:
+// until then the row's probabilities stay below 2^8, as exact in either type,
+// and o needs no rescaling.
 //
-// k_prefix_attn: warps 0-3 own a TMEM lane (query row) per thread, warp 4
-// streams 64-key tiles through a ring by TMA, warp 5 issues the products
-//   S = Q K^T (128 x 64, f32 in TMEM, two buffers), O += P V (128 x hd in TMEM)
-// with P, rounded to the keys' type, written over S.  Two blocks share an SM, so
-// one's softmax runs under the other's products and copies.  The running maximum
-// is raised only when a row's has grown by more than 2^8: until then the row's
-// P stay below 2^8, exact enough in either type, and O needs no rescaling.
+// Rows of one sequence may see different last tokens (rows > 1).  k_own takes
+// only the tokens that all rows see; the up to rows - 1 behind them go to k_join,
+// in f32, so a masked value never meets a zero probability in a product (0 x
+// NaN).  Value rows behind the last token are zeroed in shared memory for the
+// same reason.
 //
-// Rows of one own block may see different last tokens (rows > 1).  The blocks
-// take only the tokens that all rows see; the up to rows - 1 behind them go to
-// k_prefix_join, in f32, so a masked value never meets a zero probability in a
-// product (0 x NaN).  Value rows behind the last token are zeroed in shared
-// memory for the same reason.
+// k_own does not read what k_shared writes, so it starts as k_shared's blocks
+// end: it is launched as its dependent, k_shared releases it only behind its own
+// wait for earlier kernels, and one block of k_own waits for k_shared at its end,
+// so that k_join, which waits for k_own, finds both complete.
 //
-// Every wait is bounded (dc_ptx.cuh); a block whose wait gives up ends, and
-// dc_sync reports it.
+// Every wait on a barrier is bounded (dc_ptx.cuh); a block whose wait gives up
+// ends, and dc_sync reports it.
 #include <algorithm>
 
 #include "dc_cache.cuh"
@@ -39,26 +36,11 @@
 namespace {
 
 using namespace dcc;
+using dcu::F2;
 
-constexpr int ROWS = 128;      // query rows of a block: the MMA's M
-constexpr int KEYS = 64;       // keys of a tile
-constexpr int THREADS = 192;
 constexpr int MAX_ROWS = 16;
-constexpr uint32_t TMEM_COLS = 256;
-constexpr uint32_t T_O = 128;  // TMEM columns: S buffers at 0 and 64, O from here
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RAISE = 8.0f;  // growth of a row's maximum (in powers of two) that rescales it
-
-template <int NP>
-struct Cfg {
-  static constexpr int WIDTH = 64 * NP;  // head_dim, padded to panels
-  static constexpr int Q_PANEL = ROWS * 128;
-  static constexpr int KV_PANEL = KEYS * 128;
-  static constexpr int TILE = NP * KV_PANEL;
-  // 80 KB of ring beside Q's 16 NP KB: two blocks an SM (227 KB)
-  static constexpr int STAGES = NP == 2 ? 5 : 10;
-  static constexpr int SMEM = NP * Q_PANEL + STAGES * TILE + 256;
-};
 
 struct PaArgs {
   const void *q, *k_own, *v_own;
@@ -72,14 +54,18 @@ struct PaArgs {
   float c;  // scale * log2 e
   int batch, rows, heads, kv_heads, group, hd, prefix, own_max;
   int pre_rows, pre_m, pre_chunk, pre_splits;  // rows a head, row tiles, keys a split, splits
+  int pre_halves;                              // parts of a split (2 where a row tile has a block of its own)
   int own_rows, own_m, own_chunk, own_splits;
-  int pre_blocks;
   int64_t own_base;  // first own part
   int* status;
 };
 
-// Bytes of a row of the (128-byte swizzled) Q panel: 16-byte chunk ch of row r.
-__device__ __forceinline__ uint32_t swz(int r, int ch) { return (uint32_t)(r * 128 + ((ch ^ (r & 7)) << 4)); }
+// Place of row g of a head's rows (own: of one sequence; else of the batch) in q.
+__device__ __forceinline__ int64_t q_place(const PaArgs& a, int h, int g, int seq) {
+  const int rr = g / a.group;
+  const int b = seq >= 0 ? seq : rr / a.rows, r = seq >= 0 ? rr : rr - b * a.rows;
+  return b * a.q_seq + r * a.q_row + (int64_t)(h * a.group + g - rr * a.group) * a.q_head;
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -95,63 +81,70 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
   return __all_sync(~0u, dcp::mbar_wait(bar, parity, status));
 }
+// The same for two barriers at once: a wait that is met costs a hundred cycles and more.
+__device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py, int* status) {
+  const bool odd = threadIdx.x & 1;
+  return warp_wait(odd ? y : x, odd ? py : px, status);
+}
 
-// Position of tile i's keys and values in the ring's order K0 K1 V0 K2 V1 ... of n tiles.
-__device__ __forceinline__ int seq_k(int i) { return i ? 2 * i - 1 : 0; }
-__device__ __forceinline__ int seq_v(int i, int n) { return i + 1 < n ? 2 * i + 2 : 2 * n - 1; }
+// ---- the shared prefix ----------------------------------------------------------
+// Two groups of four warps take the softmax of a 128 x 128 tile of scores, a
+// thread a query row (TMEM lane); warp 8 streams 128-key tiles through a ring by
+// TMA, warp 9 issues the products
+//   S = Q K^T (128 x 128, f32 in TMEM),  O += P V (128 x hd in TMEM)
+// with P, rounded to the keys' type, written over S.  With two tiles of rows
+// each group has its own and both use each tile of keys; a tile of rows that is
+// left over has a block whose groups take every other tile of keys, and its own
+// part of the result each.  One group's softmax runs under the other's products.
+//
+// One block an SM (224 KB, all 512 TMEM columns).  Per 128 x 128 tile and SM the
+// exponential unit needs 1024 cycles, the products 500 + 500, shared memory
+// 512 + 256 for their operands and 256 for the copies: with 64-key tiles in two
+// smaller blocks an SM the operands and copies alone took 1536 (measured 1975
+// cycles a tile).
+constexpr int ROWS = 128;  // query rows of a group: the MMA's M
+constexpr int KEYS = 128;  // keys of a tile
+constexpr int SH_THREADS = 320;
+constexpr uint32_t T_O = 256;  // TMEM columns: scores at 0 and 128, O from here
+
+template <int NP>
+struct Shared {
+  static constexpr int WIDTH = 64 * NP;  // head_dim, padded to panels
+  static constexpr int PANEL = 128 * 128;
+  static constexpr int TILE = NP * PANEL;
+  static constexpr int STAGES = NP == 2 ? 5 : 8;
+  static constexpr int SMEM = (2 + STAGES) * TILE + 256;
+};
 
 template <int NP, bool BF16>
-__global__ void __launch_bounds__(THREADS, 2)
-    k_prefix_attn(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
-                  const __grid_constant__ CUtensorMap map_ko, const __grid_constant__ CUtensorMap map_vo,
-                  const __grid_constant__ PaArgs a) {
-  using C = Cfg<NP>;
+__global__ void __launch_bounds__(SH_THREADS, 1)
+    k_shared(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+             const __grid_constant__ PaArgs a) {
+  using C = Shared<NP>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
-  uint8_t* ring = smem + NP * C::Q_PANEL;
+  uint8_t* ring = smem + 2 * C::TILE;
   uint64_t* full = (uint64_t*)(ring + C::STAGES * C::TILE);
   uint64_t* empty = full + C::STAGES;
-  uint64_t* s_full = empty + C::STAGES;  // [2] scores of a buffer are in TMEM
+  uint64_t* s_full = empty + C::STAGES;  // [2] a group's scores are in TMEM
   uint64_t* p_ready = s_full + 2;        // [2] its probabilities are
-  uint64_t* o_done = p_ready + 2;        // O holds tile i
-  uint64_t* q_ready = o_done + 1;
-  uint32_t* slot = (uint32_t*)(q_ready + 1);
+  uint64_t* o_done = p_ready + 2;        // [2] its O holds the tile
+  uint64_t* q_ready = o_done + 2;        // [2]
+  uint32_t* slot = (uint32_t*)(q_ready + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // ---- this block's rows and keys
-  const bool own = (int)blockIdx.x >= a.pre_blocks;
-  int h, m, seq = 0, k0, k1, nrows;
-  int64_t part;  // of row 0 of this block's rows
-  if (!own) {
-    // row tiles of the same keys are neighbours: they read them out of L2
-    m = blockIdx.x % a.pre_m;
-    const int t = blockIdx.x / a.pre_m;
-    h = t % a.kv_heads;
-    const int split = t / a.kv_heads;
-    k0 = split * a.pre_chunk;
-    k1 = min(a.prefix, k0 + a.pre_chunk);
-    nrows = min(ROWS, a.pre_rows - m * ROWS);
-    part = (int64_t)t * a.pre_rows + m * ROWS;
-  } else {
-    int t = blockIdx.x - a.pre_blocks;
-    m = t % a.own_m;
-    t /= a.own_m;
-    const int split = t % a.own_splits, bh = t / a.own_splits;
-    h = bh % a.kv_heads;
-    seq = bh / a.kv_heads;
-    const int n = max(0, min(a.lens[seq], a.own_max) - (a.rows - 1));  // tokens that all rows see
-    k0 = split * a.own_chunk;
-    k1 = min(n, k0 + a.own_chunk);
-    nrows = min(ROWS, a.own_rows - m * ROWS);
-    part = a.own_base + (int64_t)t * a.own_rows + m * ROWS;
-  }
-  if (k1 <= k0) {
-    if ((int)threadIdx.x < nrows) a.part_ml[part + threadIdx.x] = make_float2(-INFINITY, 0.0f);
-    return;
-  }
+  // this block's rows and keys; blocks of the same keys are neighbours and read
+  // them out of L2
+  const int pairs = (a.pre_m + 1) / 2;
+  const int pair = blockIdx.x % pairs, t = blockIdx.x / pairs;
+  const int h = t % a.kv_heads, split = t / a.kv_heads;
+  const int k0 = split * a.pre_chunk, k1 = min(a.prefix, k0 + a.pre_chunk);
   const int n = (k1 - k0 + KEYS - 1) / KEYS;
+  const bool two = 2 * pair + 1 < a.pre_m;  // two tiles of rows
+  // tiles of keys: all for both groups, or every other
+  const int stride = two ? 1 : 2;
+  const int count0 = two ? n : (n + 1) / 2, count1 = two ? n : n / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; i++) {
@@ -161,12 +154,12 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int i = 0; i < 2; i++) {
       dcp::mbar_init(&s_full[i], 1);
       dcp::mbar_init(&p_ready[i], 4);
+      dcp::mbar_init(&o_done[i], 1);
+      dcp::mbar_init(&q_ready[i], 4);
     }
-    dcp::mbar_init(o_done, 1);
-    dcp::mbar_init(q_ready, 4);
     dcp::mbar_fence_init();
   }
-  if (warp == 5) dcu::alloc(slot, TMEM_COLS);
+  if (warp == 9) dcu::alloc(slot, 512);
   dcu::fence_before();
   __syncthreads();
   dcu::fence_after();
@@ -175,211 +168,460 @@ __global__ void __launch_bounds__(THREADS, 2)
   // what a block of this grid still has to get)
   asm volatile("griddepcontrol.launch_dependents;");
 
-  if (warp == 4) {
+  // Place of tile i's keys and values in the ring's order, the order of first use:
+  // K0 V0 K1 V1 .. where both groups use each tile, else K0 K1 V0 K2 V1 K3 ..
+  auto place_k = [&](int i) { return two ? 2 * i : i ? 2 * i - 1 : 0; };
+  auto place_v = [&](int i) { return two ? 2 * i + 1 : i + 1 < n ? 2 * i + 2 : 2 * n - 1; };
+
+  if (warp == 8) {
     if (lane == 0) {
-      // ---- copies: a K or V tile for each position of the ring's order
+      // ---- copies
       int issued = 0;
       for (int s = 0; s < 2 * n; s++, issued++) {
         const int st = s % C::STAGES;
         if (s >= C::STAGES && !dcp::mbar_wait(&empty[st], ((s / C::STAGES) & 1) ^ 1, a.status)) break;
-        const bool is_k = s == 0 || ((s & 1) && s != 2 * n - 1);
-        const int tile = s == 0 ? 0 : is_k ? (s + 1) / 2 : s == 2 * n - 1 ? n - 1 : s / 2 - 1;
-        const int key = k0 + tile * KEYS;
+        const bool is_k = two ? !(s & 1) : s == 0 || ((s & 1) && s != 2 * n - 1);
+        const int tile = two ? s / 2 : s == 0 ? 0 : is_k ? (s + 1) / 2 : s == 2 * n - 1 ? n - 1 : s / 2 - 1;
         dcp::mbar_expect_tx(&full[st], C::TILE);
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-          uint8_t* dst = ring + st * C::TILE + p * C::KV_PANEL;
-          if (own)
-            dcu::tma_load_4d(dst, is_k ? &map_ko : &map_vo, p * 64, h, key, seq, &full[st]);
-          else
-            dcu::tma_load_3d(dst, is_k ? &map_kp : &map_vp, p * 64, h, key, &full[st]);
-        }
+        for (int p = 0; p < NP; p++)
+          dcu::tma_load_3d(ring + st * C::TILE + p * C::PANEL, is_k ? &map_k : &map_v, p * 64, h, k0 + tile * KEYS,
+                           &full[st]);
       }
       // (given up: what is in flight lands before the block's memory goes away)
       if (issued < 2 * n)
         for (int s = max(0, issued - C::STAGES); s < issued; s++)
           dcp::mbar_wait(&full[s % C::STAGES], (s / C::STAGES) & 1, a.status);
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      // ---- products
-      constexpr uint32_t id_s = dcu::idesc(BF16, KEYS, false), id_o = dcu::idesc(BF16, C::WIDTH, true);
-      const uint32_t q_at = dcp::smem_u32(sQ), ring_at = dcp::smem_u32(ring);
-      bool ok = dcp::mbar_wait(q_ready, 0, a.status);
-      auto scores = [&](int i) {
-        const int s = seq_k(i), st = s % C::STAGES;
-        if (!dcp::mbar_wait(&full[st], (s / C::STAGES) & 1, a.status)) return false;
-        dcu::fence_after();
+  } else if (warp == 9) {
+    // ---- products, issued by lane 0: of each group in turn, P V of a tile and
+    // the scores of its next one
+    constexpr uint32_t id_s = dcu::idesc(BF16, KEYS, false), id_o = dcu::idesc(BF16, C::WIDTH, true);
+    const uint64_t dq = dcu::desc(dcp::smem_u32(sQ), 0), dk = dcu::desc(dcp::smem_u32(ring), 0);
+    const uint64_t dv = dcu::desc(dcp::smem_u32(ring), C::PANEL);
+    // Scores of group g's tile j, once the product of its tile before has read
+    // the probabilities that lie there.
+    auto scores = [&](int g, int j) {
+      const int s = place_k(two ? j : g + 2 * j), st = s % C::STAGES;
+      uint64_t* other = j ? &o_done[g] : &q_ready[two ? g : 0];
+      if (!warp_wait2(&full[st], (s / C::STAGES) & 1, other, j ? (j - 1) & 1 : 0, a.status)) return false;
+      dcu::fence_after();
+      if (lane == 0) {
+        const uint64_t k = dk + st * (C::TILE >> 4), q = dq + (two ? g : 0) * (C::TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 4 * NP; kk++)
-          dcu::mma_ss(tmem + (i & 1) * KEYS, dcu::desc(q_at + (kk >> 2) * C::Q_PANEL + (kk & 3) * 32, 0),
-                      dcu::desc(ring_at + st * C::TILE + (kk >> 2) * C::KV_PANEL + (kk & 3) * 32, 0), id_s, kk > 0);
-        dcu::commit(&empty[st]);
-        dcu::commit(&s_full[i & 1]);
-        return true;
-      };
-      ok = ok && scores(0);
-      for (int i = 0; i < n && ok; i++) {
-        if (i + 1 < n) {
-          // scores i + 1 go where the probabilities of i - 1 are read
-          if (i > 0) ok = dcp::mbar_wait(o_done, (i - 1) & 1, a.status);
-          ok = ok && scores(i + 1);
+        for (int kk = 0; kk < 4 * NP; kk++) {
+          const uint32_t off = ((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4;
+          dcu::mma_ss(tmem + g * KEYS, q + off, k + off, id_s, kk > 0);
         }
-        ok = ok && dcp::mbar_wait(&p_ready[i & 1], (i >> 1) & 1, a.status);
-        const int s = seq_v(i, n), st = s % C::STAGES;
-        ok = ok && dcp::mbar_wait(&full[st], (s / C::STAGES) & 1, a.status);
+        dcu::commit(&s_full[g]);
+        if (!two || g == 1) dcu::commit(&empty[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = scores(0, 0) && (count1 == 0 || scores(1, 0));
+    for (int j = 0; j < count0 && ok; j++) {
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
+        if (!ok || j >= (g ? count1 : count0)) continue;
+        const int s = place_v(two ? j : g + 2 * j), st = s % C::STAGES;
+        ok = warp_wait2(&p_ready[g], j & 1, &full[st], (s / C::STAGES) & 1, a.status);
         if (!ok) break;
         dcu::fence_after();
+        if (lane == 0) {
+          const uint64_t v = dv + st * (C::TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < KEYS / 16; kk++)
-          dcu::mma_ts(tmem + T_O, tmem + (i & 1) * KEYS + kk * 8,
-                      dcu::desc(ring_at + st * C::TILE + kk * 16 * 128, C::KV_PANEL), id_o, i > 0 || kk > 0);
-        dcu::commit(&empty[st]);
-        dcu::commit(o_done);
+          for (int kk = 0; kk < KEYS / 16; kk++)
+            dcu::mma_ts(tmem + T_O + g * 128, tmem + g * KEYS + kk * 8, v + (kk * 16 * 128 >> 4), id_o, j > 0 || kk > 0);
+          dcu::commit(&o_done[g]);
+          if (!two || g == 1) dcu::commit(&empty[st]);
+        }
+        __syncwarp();
+        if (j + 1 < (g ? count1 : count0)) ok = scores(g, j + 1);
       }
     }
   } else {
-    // ---- Q into shared memory, 32 rows a warp: lane's own row's place, then
-    // rows by turns
-    {
-      const int row = warp * 32 + lane;
-      int64_t at = -1;
-      if (row < nrows) {
-        const int g = row + m * ROWS, rr = g / a.group;
-        const int b = own ? seq : rr / a.rows, r = own ? rr : rr - b * a.rows;
-        at = b * a.q_seq + r * a.q_row + (int64_t)(h * a.group + g - rr * a.group) * a.q_head;
-      }
+    const int g = warp >> 2, quarter = warp & 3;  // group, TMEM lanes
+    const int m = 2 * pair + (two ? g : 0);
+    const int nrows = min(ROWS, a.pre_rows - m * ROWS);
+    // ---- Q into shared memory: each lane its own row's place, then rows by
+    // turns.  (One tile of rows: the first group's warps bring it.)
+    if (two || g == 0) {
+      const int row = quarter * 32 + lane;
+      const int64_t at = row < nrows ? q_place(a, h, row + m * ROWS, -1) : -1;
       constexpr int CH = 8 * NP, PER = 32 / CH;  // 16-byte chunks of a row, rows at once
       const int ch = lane % CH;
-#pragma unroll
+      uint8_t* dst = sQ + g * C::TILE + (ch >> 3) * C::PANEL;
+#pragma unroll 8
       for (int it = 0; it < 32 / PER; it++) {
-        const int rl = it * PER + lane / CH;
+        const int rl = it * PER + lane / CH, r = quarter * 32 + rl;
         const int64_t src = __shfl_sync(~0u, at, rl);
         uint4 v = make_uint4(0, 0, 0, 0);
         if (src >= 0 && ch * 8 < a.hd) v = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + src + ch * 8);
-        *reinterpret_cast<uint4*>(sQ + (ch >> 3) * C::Q_PANEL + swz(warp * 32 + rl, ch & 7)) = v;
+        *reinterpret_cast<uint4*>(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) dcp::mbar_arrive(q_ready);
+      if (lane == 0) dcp::mbar_arrive(&q_ready[g]);
     }
-    // ---- softmax: this thread's query row is TMEM lane warp * 32 + lane
-    const uint32_t lane_at = tmem + ((uint32_t)(warp * 32) << 16);
-    const bool used = warp * 32 < nrows;  // (a warp without rows only keeps the barriers going)
-    float mx = -INFINITY, l = 0.0f;       // the maximum in use (scores before c), the sum
+    // ---- softmax: this thread's query row is TMEM lane quarter * 32 + lane
+    const uint32_t s_at = tmem + ((uint32_t)(quarter * 32) << 16) + g * KEYS;
+    const uint32_t o_at = tmem + ((uint32_t)(quarter * 32) << 16) + T_O + g * 128;
+    const bool used = quarter * 32 < nrows;  // (a warp without rows only keeps the barriers going)
+    const int count = g ? count1 : count0;
+    float mx = -INFINITY, l = 0.0f;  // the maximum in use (scores before c), the sum
     bool ok = true;
-    for (int i = 0; i < n; i++) {
-      if (!warp_wait(&s_full[i & 1], (i >> 1) & 1, a.status)) { ok = false; break; }
+    for (int j = 0; j < count; j++) {
+      if (!warp_wait(&s_full[g], j & 1, a.status)) { ok = false; break; }
       dcu::fence_after();
-      const int nv = min(KEYS, k1 - k0 - i * KEYS);
       if (used) {
-        uint32_t s0[32], s1[32];
-        dcu::ld32(lane_at + (i & 1) * KEYS, s0);
-        dcu::ld32(lane_at + (i & 1) * KEYS + 32, s1);
-        dcu::wait_ld(s0);
-        dcu::wait_ld(s1);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int x = 0; x < 4; x++) dcu::ld32(s_at + x * 32, s[x]);
+#pragma unroll
+        for (int x = 0; x < 4; x++) dcu::wait_ld(s[x]);
+        const int nv = k1 - k0 - (two ? j : g + 2 * j) * KEYS;  // keys of the tile
         if (nv < KEYS) {
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
-            if (j >= nv) s0[j] = __float_as_uint(-INFINITY);
-            if (j + 32 >= nv) s1[j] = __float_as_uint(-INFINITY);
-          }
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int y = 0; y < 32; y++)
+              if (x * 32 + y >= nv) s[x][y] = __float_as_uint(-INFINITY);
         }
-        float t[8];
+        float top8[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) t[j] = fmaxf(__uint_as_float(s0[j]), __uint_as_float(s1[j]));
+        for (int y = 0; y < 8; y++) top8[y] = fmaxf(__uint_as_float(s[0][y]), __uint_as_float(s[1][y]));
 #pragma unroll
-        for (int j = 8; j < 32; j++) t[j & 7] = fmaxf(t[j & 7], fmaxf(__uint_as_float(s0[j]), __uint_as_float(s1[j])));
-        const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
-        if (i == 0) {
+        for (int y = 0; y < 8; y++) top8[y] = fmaxf(top8[y], fmaxf(__uint_as_float(s[2][y]), __uint_as_float(s[3][y])));
+#pragma unroll
+        for (int y = 8; y < 32; y++) {
+          top8[y & 7] = fmaxf(top8[y & 7], fmaxf(__uint_as_float(s[0][y]), __uint_as_float(s[1][y])));
+          top8[y & 7] = fmaxf(top8[y & 7], fmaxf(__uint_as_float(s[2][y]), __uint_as_float(s[3][y])));
+        }
+        const float top = fmaxf(fmaxf(fmaxf(top8[0], top8[1]), fmaxf(top8[2], top8[3])),
+                                fmaxf(fmaxf(top8[4], top8[5]), fmaxf(top8[6], top8[7])));
+        if (j == 0) {
           mx = top;
         } else if (__any_sync(~0u, top > mx && !((top - mx) * a.c <= RAISE))) {
-          // O *= 2^(c (old - new)) once the product of tile i - 1 is in it
+          // O *= 2^(c (old - new)).  (These scores were issued behind the end of
+          // the product of the tile before: O holds it, and nothing writes O.)
           const float up = fmaxf(mx, top);
           const float f = mx == -INFINITY ? 0.0f : mx == up ? 1.0f : dcu::ex2((mx - up) * a.c);
           mx = up;
           l *= f;
-          // (scores i were issued after product i - 2 was done, so this parity
-          // can only mean product i - 1)
-          if (!warp_wait(o_done, (i - 1) & 1, a.status)) { ok = false; break; }
-          dcu::fence_after();
 #pragma unroll 1
-          for (int col = 0; col < C::WIDTH; col += 32) {
-            uint32_t o[32];
-            dcu::ld32(lane_at + T_O + col, o);
+          for (int col = 0; col < C::WIDTH; col += 16) {
+            uint32_t o[16];
+            dcu::ld16(o_at + col, o);
             dcu::wait_ld(o);
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            dcu::st32(lane_at + T_O + col, o);
+            for (int y = 0; y < 16; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            dcu::st16(o_at + col, o);
           }
           dcu::wait_st();
         }
         const float base = mx == -INFINITY ? 0.0f : mx * a.c;
-        float ls[4] = {0, 0, 0, 0};
-        uint32_t p[32];
+        const F2 c2 = dcu::f2(a.c, a.c), b2 = dcu::f2(-base, -base);
+        F2 sum[2] = {dcu::f2(0, 0), dcu::f2(0, 0)};
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-          const float e0 = dcu::ex2(fmaf(__uint_as_float(s0[2 * j]), a.c, -base));
-          const float e1 = dcu::ex2(fmaf(__uint_as_float(s0[2 * j + 1]), a.c, -base));
-          const float e2 = dcu::ex2(fmaf(__uint_as_float(s1[2 * j]), a.c, -base));
-          const float e3 = dcu::ex2(fmaf(__uint_as_float(s1[2 * j + 1]), a.c, -base));
-          ls[0] += e0, ls[1] += e1, ls[2] += e2, ls[3] += e3;
-          // (the sum keeps the unrounded values: lse is exact to f32; P is
-          // rounded to the type of the products' operands, half a step each)
-          p[j] = pack2<BF16>(e0, e1);
-          p[16 + j] = pack2<BF16>(e2, e3);
+        for (int x = 0; x < 4; x += 2) {
+          uint32_t p[32];
+#pragma unroll
+          for (int y = 0; y < 32; y++) {
+            // (the sum keeps the unrounded values: lse is exact to f32; P is
+            // rounded to the type of the products' operands, half a step each)
+            const uint32_t(&u)[32] = s[x + y / 16];
+            const int k = (y % 16) * 2;
+            const float2 e = dcu::split(dcu::fma2(dcu::f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, b2));
+            const float e0 = dcu::ex2(e.x), e1 = dcu::ex2(e.y);
+            sum[y & 1] = dcu::add2(sum[y & 1], dcu::f2(e0, e1));
+            p[y] = pack2<BF16>(e0, e1);
+          }
+          dcu::st32(s_at + x * 16, p);
         }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        dcu::st32(lane_at + (i & 1) * KEYS, p);
+        const float2 both = dcu::split(dcu::add2(sum[0], sum[1]));
+        l += both.x + both.y;
         dcu::wait_st();
-      }
-      if (own && nv < KEYS) {
-        // value rows behind the last token hold anything: zero them
-        const int s = seq_v(i, n), st = s % C::STAGES;
-        if (!warp_wait(&full[st], (s / C::STAGES) & 1, a.status)) { ok = false; break; }
-        uint8_t* v = ring + st * C::TILE;
-        for (int j = threadIdx.x; j < (KEYS - nv) * 8 * NP; j += 128) {
-          const int p = j / ((KEYS - nv) * 8), rest = j - p * (KEYS - nv) * 8;
-          *reinterpret_cast<uint4*>(v + p * C::KV_PANEL + nv * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       dcu::fence_before();
       __syncwarp();
-      if (lane == 0) dcp::mbar_arrive(&p_ready[i & 1]);
+      if (lane == 0) dcp::mbar_arrive(&p_ready[g]);
     }
-    // (one product after the other: a parity alone cannot tell n - 1 from n - 3)
-    if (ok && used && (n < 2 || warp_wait(o_done, (n - 2) & 1, a.status)) && warp_wait(o_done, (n - 1) & 1, a.status)) {
-      dcu::fence_after();
-      const int row = warp * 32 + lane;
-      float* dst = a.part_o + (part + row) * C::WIDTH;
+    if (used) {
+      const int row = quarter * 32 + lane;
+      const int half = two ? 0 : g;
+      const int64_t part = ((int64_t)(split * a.pre_halves + half) * a.kv_heads + h) * a.pre_rows + m * ROWS + row;
+      if (count > 0 && ok && warp_wait(&o_done[g], (count - 1) & 1, a.status)) {
+        dcu::fence_after();
+        float* dst = a.part_o + part * C::WIDTH;
 #pragma unroll 1
-      for (int col = 0; col < C::WIDTH; col += 32) {
-        uint32_t o[32];
-        dcu::ld32(lane_at + T_O + col, o);
-        dcu::wait_ld(o);
-        if (row < nrows) {
+        for (int col = 0; col < C::WIDTH; col += 32) {
+          uint32_t o[32];
+          dcu::ld32(o_at + col, o);
+          dcu::wait_ld(o);
+          if (row < nrows) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(dst + col + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int y = 0; y < 32; y += 4)
+              *reinterpret_cast<uint4*>(dst + col + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+          }
         }
+      } else {
+        mx = -INFINITY, l = 0.0f;
       }
-      if (row < nrows) a.part_ml[part + row] = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
+      if (row < nrows) a.part_ml[part] = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
     }
     dcu::fence_before();
   }
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     dcu::fence_after();
-    dcu::dealloc(tmem, TMEM_COLS);
+    dcu::dealloc(tmem, 512);
   }
 }
 
-// One warp per (sequence, row, query head): joins the parts of its row, and
-// scores the own tokens behind those that all rows see.  A lane holds WIDTH / 32
-// channels.
+// ---- each sequence's own keys ----------------------------------------------------
+// Up to 16 query rows a block (row, head of the group), mostly four to eight, so
+// the work is the reading of keys and values: HBM-bound.  Each of four warps
+// streams its own 16-key tiles (TMA, three in flight, 24 KB a warp: 192 KB an SM
+// over two blocks) and keeps its own running maximum, sum and output in registers,
+// with 16 x 8 x 16 products (a tcgen05 tile of 128 rows would be empty but for
+// these, and its round trips through TMEM cost more than the copies: 41 us
+// against HBM's 21 for 64 sequences of up to 1024 tokens).  The warps' results
+// join in shared memory.
+constexpr int OWN_ROWS = 16;
+constexpr int OWN_KEYS = 16;
+constexpr int OWN_WARPS = 4;
+constexpr int OWN_STAGES = 3;
+constexpr int OWN_STEP = OWN_KEYS * OWN_WARPS;
+
+template <int NP>
+struct Own {
+  static constexpr int WIDTH = 64 * NP;
+  static constexpr int PANEL = OWN_KEYS * 128;
+  static constexpr int TILE = NP * PANEL;
+  static constexpr int WARP = OWN_STAGES * 2 * TILE;  // a warp's ring
+  static constexpr int SMEM = OWN_WARPS * WARP + 128;
+  static_assert(WARP >= OWN_ROWS * (WIDTH + 4) * 4, "the warps' results are joined in their rings");
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// `behind`: launched behind k_shared, whose end it waits for last.
+template <int NP, bool BF16>
+__global__ void __launch_bounds__(OWN_WARPS * 32, 2)
+    k_own(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+          const __grid_constant__ PaArgs a, const int behind) {
+  using C = Own<NP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = (uint64_t*)(smem + OWN_WARPS * C::WARP);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (!behind) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  int t = blockIdx.x;
+  const int m = t % a.own_m;
+  t /= a.own_m;
+  const int split = t % a.own_splits, bh = t / a.own_splits, h = bh % a.kv_heads, seq = bh / a.kv_heads;
+  const int seen = max(0, min(a.lens[seq], a.own_max) - (a.rows - 1));  // tokens that all rows see
+  const int k0 = split * a.own_chunk, k1 = min(seen, k0 + a.own_chunk);
+  const int nrows = min(OWN_ROWS, a.own_rows - m * OWN_ROWS);
+  const int64_t part = a.own_base + (int64_t)t * a.own_rows + m * OWN_ROWS;
+  if (k1 <= k0) {
+    if ((int)threadIdx.x < nrows) a.part_ml[part + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+  } else {
+    uint8_t* ring = smem + warp * C::WARP;
+    uint64_t* full = bars + warp * OWN_STAGES;
+    const int tiles = (k1 - k0 + OWN_KEYS - 1) / OWN_KEYS, n = (tiles - warp + OWN_WARPS - 1) / OWN_WARPS;
+    auto key_of = [&](int i) { return k0 + (i * OWN_WARPS + warp) * OWN_KEYS; };
+    auto copy = [&](int i) {
+      const int st = i % OWN_STAGES;
+      dcp::mbar_expect_tx(&full[st], 2 * C::TILE);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        uint8_t* dst = ring + st * 2 * C::TILE + p * C::PANEL;
+        dcu::tma_load_4d(dst, &map_k, p * 64, h, key_of(i), seq, &full[st]);
+        dcu::tma_load_4d(dst + C::TILE, &map_v, p * 64, h, key_of(i), seq, &full[st]);
+      }
+    };
+    if (lane == 0) {
+      for (int i = 0; i < OWN_STAGES; i++) dcp::mbar_init(&full[i], 1);
+      dcp::mbar_fence_init();
+      for (int i = 0; i < min(n, OWN_STAGES); i++) copy(i);
+    }
+    __syncwarp();
+    // Q fragments: rows lane / 4 and + 8, channels 16 x + 2 (lane % 4) and + 8
+    uint32_t q[4 * NP][4];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int row = lane / 4 + 8 * half;
+      const uint16_t* src = (const uint16_t*)a.q + (row < nrows ? q_place(a, h, row + m * OWN_ROWS, seq) : 0);
+#pragma unroll
+      for (int x = 0; x < 4 * NP; x++)
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const int ch = 16 * x + 8 * y + 2 * (lane % 4);
+          q[x][half + 2 * y] = row < nrows && ch < a.hd ? *reinterpret_cast<const uint32_t*>(src + ch) : 0;
+        }
+    }
+    float o[8 * NP][4], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < 8 * NP; x++)
+#pragma unroll
+      for (int y = 0; y < 4; y++) o[x][y] = 0.0f;
+    bool ok = true;
+    const int key_k = (lane / 16) * 8 + lane % 8, key_v = ((lane / 8) & 1) * 8 + lane % 8;
+    for (int i = 0; i < n; i++) {
+      const int st = i % OWN_STAGES;
+      ok = warp_wait(&full[st], (i / OWN_STAGES) & 1, a.status);
+      if (!ok) break;
+      const int nv = min(OWN_KEYS, k1 - key_of(i));
+      const uint32_t k_at = dcp::smem_u32(ring + st * 2 * C::TILE), v_at = k_at + C::TILE;
+      float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int x = 0; x < 4 * NP; x++) {
+        const int ch = 2 * x + ((lane / 8) & 1);
+        uint32_t b[4];
+        ldmatrix4(b, k_at + (ch >> 3) * C::PANEL + key_k * 128 + (((ch & 7) ^ (key_k & 7)) << 4));
+        mma16816<BF16>(s[0], q[x], b[0], b[1]);
+        mma16816<BF16>(s[1], q[x], b[2], b[3]);
+      }
+      if (nv < OWN_KEYS) {
+        // value rows behind the last token hold anything: zero them
+        for (int j = lane; j < (OWN_KEYS - nv) * 8 * NP; j += 32) {
+          const int p = j / ((OWN_KEYS - nv) * 8), rest = j - p * (OWN_KEYS - nv) * 8;
+          *reinterpret_cast<uint4*>(ring + st * 2 * C::TILE + C::TILE + p * C::PANEL + nv * 128 + rest * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int y = 0; y < 4; y++)
+            if (8 * x + 2 * (lane % 4) + (y & 1) >= nv) s[x][y] = -INFINITY;
+      }
+      float top[2] = {fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
+                      fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]))};
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], 1));
+        top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], 2));
+      }
+      bool raise = false;
+#pragma unroll
+      for (int y = 0; y < 2; y++) raise |= top[y] > mx[y] && !((top[y] - mx[y]) * a.c <= RAISE);
+      if (__any_sync(~0u, raise)) {
+        float f[2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const float up = fmaxf(mx[y], top[y]);
+          f[y] = mx[y] == -INFINITY ? 0.0f : mx[y] == up ? 1.0f : dcu::ex2((mx[y] - up) * a.c);
+          mx[y] = up;
+          l[y] *= f[y];
+        }
+        if (i > 0) {
+#pragma unroll
+          for (int x = 0; x < 8 * NP; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) o[x][y] *= f[y >> 1];
+        }
+      }
+      const float base[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] * a.c, mx[1] == -INFINITY ? 0.0f : mx[1] * a.c};
+      float e[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          e[x][y] = dcu::ex2(fmaf(s[x][y], a.c, -base[y >> 1]));
+          l[y >> 1] += e[x][y];
+        }
+      const uint32_t p[4] = {pack2<BF16>(e[0][0], e[0][1]), pack2<BF16>(e[0][2], e[0][3]), pack2<BF16>(e[1][0], e[1][1]),
+                             pack2<BF16>(e[1][2], e[1][3])};
+#pragma unroll
+      for (int x = 0; x < 4 * NP; x++) {
+        const int ch = 2 * x + lane / 16;
+        uint32_t b[4];
+        ldmatrix4_t(b, v_at + (ch >> 3) * C::PANEL + key_v * 128 + (((ch & 7) ^ (key_v & 7)) << 4));
+        mma16816<BF16>(o[2 * x], p, b[0], b[1]);
+        mma16816<BF16>(o[2 * x + 1], p, b[2], b[3]);
+      }
+      __syncwarp();
+      if (lane == 0 && i + OWN_STAGES < n) copy(i + OWN_STAGES);
+    }
+    if (!ok)  // (given up: what is in flight lands before the block's memory goes away)
+      for (int i = 0; i < OWN_STAGES; i++)
+        if (i < n) dcp::mbar_wait(&full[i], 0, a.status);
+    // ---- the warps' results
+    float* mine = (float*)ring;  // 16 rows of WIDTH + 4 floats (the rows of a fragment in different banks)
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      l[y] += __shfl_xor_sync(~0u, l[y], 1);
+      l[y] += __shfl_xor_sync(~0u, l[y], 2);
+      const int row = lane / 4 + 8 * y;
+      if (lane % 4 == 0)
+        *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + C::WIDTH) =
+            make_float2(mx[y] == -INFINITY ? -INFINITY : mx[y] * a.c, l[y]);
+#pragma unroll
+      for (int x = 0; x < 8 * NP; x++)
+        *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + 8 * x + 2 * (lane % 4)) =
+            make_float2(o[x][2 * y], o[x][2 * y + 1]);
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < nrows * (C::WIDTH / 4); j += OWN_WARPS * 32) {
+      const int row = j / (C::WIDTH / 4), col = (j - row * (C::WIDTH / 4)) * 4;
+      const float* r = (const float*)smem + row * (C::WIDTH + 4);
+      float2 ml[OWN_WARPS];
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < OWN_WARPS; w++) {
+        ml[w] = *reinterpret_cast<const float2*>(r + w * (C::WARP / 4) + C::WIDTH);
+        top = fmaxf(top, ml[w].x);
+      }
+      const float base = top == -INFINITY ? 0.0f : top;
+      float4 sum = make_float4(0, 0, 0, 0);
+      float z = 0.0f;
+#pragma unroll
+      for (int w = 0; w < OWN_WARPS; w++) {
+        const float f = ml[w].y == 0.0f ? 0.0f : dcu::ex2(ml[w].x - base);
+        const float4 v = *reinterpret_cast<const float4*>(r + w * (C::WARP / 4) + col);
+        z = fmaf(f, ml[w].y, z);
+        sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y), sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
+      }
+      *reinterpret_cast<float4*>(a.part_o + (part + row) * C::WIDTH + col) = sum;
+      if (col == 0) a.part_ml[part + row] = make_float2(top, z);
+    }
+  }
+  if (behind && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ---- joining the parts ------------------------------------------------------------
+// One warp per (sequence, row, query head): joins the parts of its row, eight
+// in flight, and scores the own tokens behind those that all rows see.  A lane
+// holds WIDTH / 32 channels.
 template <int NP, typename T, typename TO>
-__global__ void __launch_bounds__(128) k_prefix_join(const __grid_constant__ PaArgs a) {
+__global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) {
   constexpr int W = 64 * NP, E = W / 32;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -388,12 +630,16 @@ __global__ void __launch_bounds__(128) k_prefix_join(const __grid_constant__ PaA
   if (id >= (int64_t)a.batch * a.rows * a.heads) return;
   const int head = id % a.heads, br = id / a.heads, r = br % a.rows, b = br / a.rows;
   const int h = head / a.group, g = head - h * a.group;
-  // parts: prefix splits, then own splits
-  const int64_t pre_at = (int64_t)h * a.pre_rows + (int64_t)br * a.group + g, pre_step = (int64_t)a.kv_heads * a.pre_rows;
+  // parts: of the prefix's splits (both halves where the row's tile has a block
+  // of its own), then of the own splits
+  const int row = br * a.group + g;
+  const int halves = a.pre_halves == 2 && row / ROWS == a.pre_m - 1 ? 2 : 1;
+  const int pre = a.pre_splits * halves, total = pre + a.own_splits;
   const int64_t own_at = a.own_base + (int64_t)(b * a.kv_heads + h) * a.own_splits * a.own_rows + r * a.group + g;
-  const int total = a.pre_splits + a.own_splits;
   auto at = [&](int i) {
-    return i < a.pre_splits ? pre_at + i * pre_step : own_at + (int64_t)(i - a.pre_splits) * a.own_rows;
+    if (i >= pre) return own_at + (int64_t)(i - pre) * a.own_rows;
+    const int64_t part = halves == 2 ? i : i * a.pre_halves;
+    return (part * a.kv_heads + h) * a.pre_rows + row;
   };
   // the tail's scores, lane j that of token j
   int tail0 = 0, tail = 0;
@@ -433,20 +679,30 @@ __global__ void __launch_bounds__(128) k_prefix_join(const __grid_constant__ PaA
     // (a part of sum 0 has no O)
     const float w = ml.y == 0.0f ? 0.0f : dcu::ex2(ml.x - base);
     L += w * ml.y;
-    const int cnt = min(32, total - i0);
     const unsigned some = __ballot_sync(~0u, ml.y != 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < cnt; i++) {
-      const float wi = __shfl_sync(~0u, w, i);
-      if (!(some >> i & 1)) continue;
-      const float* o = a.part_o + at(i0 + i) * W + c0;
-      if constexpr (E == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(o);
-        acc[0] = fmaf(wi, f.x, acc[0]), acc[1] = fmaf(wi, f.y, acc[1]);
-        acc[2] = fmaf(wi, f.z, acc[2]), acc[3] = fmaf(wi, f.w, acc[3]);
-      } else {
-        const float2 f = *reinterpret_cast<const float2*>(o);
-        acc[0] = fmaf(wi, f.x, acc[0]), acc[1] = fmaf(wi, f.y, acc[1]);
+    const int cnt = min(32, total - i0);
+    for (int i = 0; i < cnt; i += 8) {
+      float v[8][E];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[j][e] = 0.0f;
+        if (some >> (i + j) & 1) {
+          const float* o = a.part_o + at(i0 + i + j) * W + c0;
+          if constexpr (E == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(o);
+            v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(o);
+            v[j][0] = f.x, v[j][1] = f.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float wj = __shfl_sync(~0u, w, i + j);
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = fmaf(wj, v[j][e], acc[e]);
       }
     }
   }
@@ -475,43 +731,45 @@ __global__ void __launch_bounds__(128) k_prefix_join(const __grid_constant__ PaA
 // How a call's keys are split: the splits follow from sizes alone, so that the
 // workspace's size is known before the call.
 struct Plan {
-  int group, pre_rows, pre_m, pre_chunk, pre_splits, own_rows, own_m, own_chunk, own_splits;
+  int group, pre_rows, pre_m, pre_chunk, pre_splits, pre_halves, own_rows, own_m, own_chunk, own_splits;
   int64_t pre_blocks, own_blocks, own_base, parts;
   int width;
 };
+// The number of even shares of `tiles` tiles for each of `items`, `slots` blocks
+// at a time, that ends first: a block costs `start` tiles beside its own (TMEM,
+// Q, the first copy, its parts), a part about an eighth of a tile of joining.
+int shares(int64_t items, int64_t tiles, int64_t slots, int64_t start) {
+  if (!items) return 1;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= std::min(tiles, 2 * slots / items + 1); s++) {
+    const int64_t waves = (items * s + slots - 1) / slots;
+    const int64_t end = 8 * waves * (start + (tiles + s - 1) / s) + s;
+    if (end < least) least = end, best = s;
+  }
+  return (int)best;
+}
 Plan make_plan(const dc_prefix_attn& A, int sm_count) {
   Plan p = {};
   p.group = A.heads / A.kv_heads;
   p.width = A.head_dim <= 64 ? 64 : 128;
-  p.pre_rows = A.batch * A.rows * p.group;
-  p.pre_m = (p.pre_rows + ROWS - 1) / ROWS;
-  p.own_rows = A.rows * p.group;
-  p.own_m = (p.own_rows + ROWS - 1) / ROWS;
-  const int64_t tp = (A.prefix + KEYS - 1) / KEYS, to = (A.own_max + KEYS - 1) / KEYS;
-  const int64_t hp = (int64_t)A.kv_heads * p.pre_m, ho = (int64_t)A.batch * A.kv_heads * p.own_m;
-  // One wave: two blocks an SM.  Tiles a block (own caches count as half full)
-  // from the whole work, but not fewer than four, over which a block's start
-  // (TMEM, Q, the first copy) is spread.
-  const int64_t slots = 2 * (int64_t)sm_count;
-  int64_t per = std::max<int64_t>(4, (hp * tp + ho * ((to + 1) / 2) + slots - 1) / slots);
-  // (a second wave is not worth starting for a few blocks; where the sequences'
-  // own blocks alone are more than one wave, they queue behind the prefix's)
-  for (; hp + ho <= slots; per += (per + 7) / 8) {
-    const int64_t sp = (tp + per - 1) / per, so = (to + 2 * per - 1) / (2 * per);
-    if (hp * sp + ho * so <= slots) break;
-  }
-  auto split = [](int64_t tiles, int64_t most, int* chunk) {
+  auto split = [](int64_t tiles, int shares, int tile, int* chunk) {
     if (!tiles) return *chunk = 0;
-    int64_t s = (tiles + most - 1) / most;
-    const int64_t each = (tiles + s - 1) / s;  // even shares
-    *chunk = (int)(each * KEYS);
+    const int64_t each = (tiles + shares - 1) / shares;
+    *chunk = (int)(each * tile);
     return (int)((tiles + each - 1) / each);
   };
-  p.pre_splits = split(tp, per, &p.pre_chunk);
-  p.own_splits = split(to, 2 * per, &p.own_chunk);
+  p.pre_rows = A.batch * A.rows * p.group;
+  p.pre_m = (p.pre_rows + ROWS - 1) / ROWS;
+  p.pre_halves = 1 + (p.pre_m & 1);
+  const int64_t tp = (A.prefix + KEYS - 1) / KEYS, hp = (int64_t)A.kv_heads * ((p.pre_m + 1) / 2);
+  p.pre_splits = split(tp, shares(hp, tp, sm_count, 3), KEYS, &p.pre_chunk);
+  p.own_rows = A.rows * p.group;
+  p.own_m = (p.own_rows + OWN_ROWS - 1) / OWN_ROWS;
+  const int64_t to = (A.own_max + OWN_STEP - 1) / OWN_STEP, ho = (int64_t)A.batch * A.kv_heads * p.own_m;
+  p.own_splits = split(to, shares(ho, to, 2 * sm_count, 4), OWN_STEP, &p.own_chunk);
   p.pre_blocks = hp * p.pre_splits;
   p.own_blocks = ho * p.own_splits;
-  p.own_base = (int64_t)p.pre_splits * A.kv_heads * p.pre_rows;
+  p.own_base = (int64_t)p.pre_splits * p.pre_halves * A.kv_heads * p.pre_rows;
   p.parts = p.own_base + (int64_t)A.batch * A.kv_heads * p.own_splits * p.own_rows;
   return p;
 }
@@ -536,15 +794,19 @@ int check(dc_ctx* ctx, const dc_prefix_attn& A) {
 size_t ws_bytes_of(const Plan& p) { return (size_t)p.parts * (p.width * 4 + 8); }
 
 template <int NP, bool BF16>
-int run(dc_ctx* ctx, const CUtensorMap (&maps)[4], const PaArgs& a, int64_t blocks, bool f32_out) {
+int run(dc_ctx* ctx, const CUtensorMap (&maps)[4], const PaArgs& a, const Plan& p, bool f32_out) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  if (blocks)
-    if (int rc = launch(ctx, k_prefix_attn<NP, BF16>, dim3((unsigned)blocks), THREADS, Cfg<NP>::SMEM, 1, maps[0],
-                        maps[1], maps[2], maps[3], a))
+  if (p.pre_blocks)
+    if (int rc = launch(ctx, k_shared<NP, BF16>, dim3((unsigned)p.pre_blocks), SH_THREADS, Shared<NP>::SMEM, 1, maps[0],
+                        maps[1], a))
+      return rc;
+  if (p.own_blocks)
+    if (int rc = launch(ctx, k_own<NP, BF16>, dim3((unsigned)p.own_blocks), OWN_WARPS * 32, Own<NP>::SMEM, 1, maps[2],
+                        maps[3], a, (int)(p.pre_blocks > 0)))
       return rc;
   const dim3 grid((unsigned)(((int64_t)a.batch * a.rows * a.heads + 3) / 4));
-  return f32_out ? launch(ctx, k_prefix_join<NP, T, float>, grid, 128, 0, 1, a)
-                 : launch(ctx, k_prefix_join<NP, T, T>, grid, 128, 0, 1, a);
+  return f32_out ? launch(ctx, k_join<NP, T, float>, grid, 128, 0, 1, a)
+                 : launch(ctx, k_join<NP, T, T>, grid, 128, 0, 1, a);
 }
 
 }  // namespace
@@ -604,7 +866,7 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
   CUtensorMap maps[4];
   memset(maps, 0, sizeof maps);
   const uint64_t hd = A.head_dim, kv = A.kv_heads;
-  const uint32_t box[4] = {64, 1, KEYS, 1};
+  const uint32_t box[3] = {64, 1, KEYS}, own_box[4] = {64, 1, OWN_KEYS, 1};
   bool ok = true;
   if (A.prefix) {
     const uint64_t dims[3] = {hd, kv, (uint64_t)A.prefix};
@@ -616,8 +878,8 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
     const uint64_t dims[4] = {hd, kv, (uint64_t)A.own_max, (uint64_t)A.batch};
     const uint64_t sk[3] = {2 * (uint64_t)A.ko_head, 2 * (uint64_t)A.ko_tok, 2 * (uint64_t)A.ko_seq};
     const uint64_t sv[3] = {2 * (uint64_t)A.vo_head, 2 * (uint64_t)A.vo_tok, 2 * (uint64_t)A.vo_seq};
-    ok = ok && dcu::encode(&maps[2], A.k_own, bf16, 4, dims, sk, box) &&
-         dcu::encode(&maps[3], A.v_own, bf16, 4, dims, sv, box);
+    ok = ok && dcu::encode(&maps[2], A.k_own, bf16, 4, dims, sk, own_box) &&
+         dcu::encode(&maps[3], A.v_own, bf16, 4, dims, sv, own_box);
   }
   if (!ok) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: these k or v strides make no tensor map");
 
@@ -633,12 +895,12 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
   a.batch = A.batch, a.rows = A.rows, a.heads = A.heads, a.kv_heads = A.kv_heads, a.group = pl.group;
   a.hd = A.head_dim, a.prefix = A.prefix, a.own_max = A.own_max;
   a.pre_rows = pl.pre_rows, a.pre_m = pl.pre_m, a.pre_chunk = pl.pre_chunk, a.pre_splits = pl.pre_splits;
+  a.pre_halves = pl.pre_halves;
   a.own_rows = pl.own_rows, a.own_m = pl.own_m, a.own_chunk = pl.own_chunk, a.own_splits = pl.own_splits;
-  a.pre_blocks = (int)pl.pre_blocks, a.own_base = pl.own_base, a.status = ctx->d_status;
-  const int64_t blocks = pl.pre_blocks + pl.own_blocks;
-  if (blocks > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: too many blocks");
+  a.own_base = pl.own_base, a.status = ctx->d_status;
+  if (std::max(pl.pre_blocks, pl.own_blocks) > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: too many blocks");
   const bool f32_out = A.out_type == DC_F32;
   if (pl.width == 64)
-    return bf16 ? run<1, true>(ctx, maps, a, blocks, f32_out) : run<1, false>(ctx, maps, a, blocks, f32_out);
-  return bf16 ? run<2, true>(ctx, maps, a, blocks, f32_out) : run<2, false>(ctx, maps, a, blocks, f32_out);
+    return bf16 ? run<1, true>(ctx, maps, a, pl, f32_out) : run<1, false>(ctx, maps, a, pl, f32_out);
+  return bf16 ? run<2, true>(ctx, maps, a, pl, f32_out) : run<2, false>(ctx, maps, a, pl, f32_out);
 }

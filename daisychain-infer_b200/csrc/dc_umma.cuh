@@ -109,12 +109,26 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
       DCU_I8(r, 8), DCU_I8(r, 16), DCU_I8(r, 24), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : DCU_R8(r, 0), DCU_R8(r, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::DCU_I8(
+          r, 0),
+      DCU_I8(r, 8), "r"(addr)
+      : "memory");
+}
 // The loads' registers pass through the wait, so that no use of them can be
 // scheduled before it.
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+template <int N>
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
