@@ -92,20 +92,25 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // thread a query row (TMEM lane); warp 8 streams 128-key tiles through a ring by
 // TMA, warp 9 issues the products
 //   S = Q K^T (128 x 128, f32 in TMEM),  O += P V (128 x hd in TMEM)
-// with P, rounded to the keys' type, written over S.  With two tiles of rows
-// each group has its own and both use each tile of keys; a tile of rows that is
-// left over has a block whose groups take every other tile of keys, and its own
-// part of the result each.  One group's softmax runs under the other's products.
+// with P rounded to the keys' type.  With two tiles of rows each group has its
+// own and both use each tile of keys; a tile of rows that is left over has a block
+// whose groups take every other tile of keys, and its own part of the result
+// each.  One group's softmax runs under the other's products.
 //
-// One block an SM (224 KB, all 512 TMEM columns).  Per 128 x 128 tile and SM the
-// exponential unit needs 1024 cycles, the products 500 + 500, shared memory
-// 512 + 256 for their operands and 256 for the copies: with 64-key tiles in two
-// smaller blocks an SM the operands and copies alone took 1536 (measured 1975
-// cycles a tile).
+// One block an SM (224 KB, all 512 TMEM columns).  Heads up to 64 wide leave room
+// for P beside S: the next scores are formed as soon as these have been read.
+// Wider ones have P written over S, and the next scores wait for the product.
+// Either way P goes out in two halves, so that the product starts on the first.
+//
+// Per 128 x 128 tile and SM the exponential unit needs 1024 cycles (a quarter less
+// with every fourth pair taken on the multiply-add pipe), the products 500 + 500,
+// shared memory 512 + 256 for their operands and 256 for the copies: with 64-key
+// tiles in two smaller blocks an SM the operands and copies alone took 1536
+// (measured 1975 cycles a tile).
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
+constexpr int FMA_EVERY = 4;  // every fourth pair of exponentials on the multiply-add pipe
 constexpr int SH_THREADS = 320;
-constexpr uint32_t T_O = 256;  // TMEM columns: scores at 0 and 128, O from here
 
 template <int NP>
 struct Shared {
@@ -114,6 +119,11 @@ struct Shared {
   static constexpr int TILE = NP * PANEL;
   static constexpr int STAGES = NP == 2 ? 5 : 8;
   static constexpr int SMEM = (2 + STAGES) * TILE + 256;
+  // TMEM columns of group g: scores, O, probabilities
+  static constexpr bool APART = NP == 1;  // probabilities beside the scores
+  static constexpr uint32_t s_col(int g) { return g * 128; }
+  static constexpr uint32_t o_col(int g) { return 256 + g * WIDTH; }
+  static constexpr uint32_t p_col(int g) { return APART ? 384 + g * 64 : s_col(g); }
 };
 
 template <int NP, bool BF16>
@@ -127,12 +137,13 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
   uint64_t* full = (uint64_t*)(ring + C::STAGES * C::TILE);
   uint64_t* empty = full + C::STAGES;
   uint64_t* s_full = empty + C::STAGES;  // [2] a group's scores are in TMEM
-  uint64_t* p_ready = s_full + 2;        // [2] its probabilities are
-  uint64_t* o_done = p_ready + 2;        // [2] its O holds the tile
+  uint64_t* s_free = s_full + 2;         // [2] and have been read (APART)
+  uint64_t* p_ready = s_free + 2;        // [2 x 2] half of its probabilities are in TMEM
+  uint64_t* o_done = p_ready + 4;        // [2] its O holds the tile
   uint64_t* q_ready = o_done + 2;        // [2]
   uint32_t* slot = (uint32_t*)(q_ready + 2);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // this block's rows and keys; blocks of the same keys are neighbours and read
   // them out of L2
@@ -153,7 +164,9 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     }
     for (int i = 0; i < 2; i++) {
       dcp::mbar_init(&s_full[i], 1);
-      dcp::mbar_init(&p_ready[i], 4);
+      dcp::mbar_init(&s_free[i], 4);
+      dcp::mbar_init(&p_ready[2 * i], 4);
+      dcp::mbar_init(&p_ready[2 * i + 1], 4);
       dcp::mbar_init(&o_done[i], 1);
       dcp::mbar_init(&q_ready[i], 4);
     }
@@ -163,7 +176,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
   dcu::fence_before();
   __syncthreads();
   dcu::fence_after();
-  const uint32_t tmem = *slot;
+  const uint32_t tmem = dcu::uniform(*slot);
   // (only now: a dependent that takes TMEM before its own wait must not take
   // what a block of this grid still has to get)
   asm volatile("griddepcontrol.launch_dependents;");
@@ -194,27 +207,27 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           dcp::mbar_wait(&full[s % C::STAGES], (s / C::STAGES) & 1, a.status);
     }
   } else if (warp == 9) {
-    // ---- products, issued by lane 0: of each group in turn, P V of a tile and
-    // the scores of its next one
+    // ---- products, of the groups by turns: that keeps their softmaxes half a
+    // tile apart (with a warp for each group they fell into step, and waited
+    // for the tensor pipe and the exponential unit at the same times)
     constexpr uint32_t id_s = dcu::idesc(BF16, KEYS, false), id_o = dcu::idesc(BF16, C::WIDTH, true);
-    const uint64_t dq = dcu::desc(dcp::smem_u32(sQ), 0), dk = dcu::desc(dcp::smem_u32(ring), 0);
-    const uint64_t dv = dcu::desc(dcp::smem_u32(ring), C::PANEL);
-    // Scores of group g's tile j, once the product of its tile before has read
-    // the probabilities that lie there.
+    const uint64_t dq = dcu::desc(dcp::smem_u32(sQ), 0);
+    const uint64_t dk = dcu::desc(dcp::smem_u32(ring), 0), dv = dcu::desc(dcp::smem_u32(ring), C::PANEL);
     auto scores = [&](int g, int j) {
       const int s = place_k(two ? j : g + 2 * j), st = s % C::STAGES;
-      uint64_t* other = j ? &o_done[g] : &q_ready[two ? g : 0];
+      // the scores before have been read; where the probabilities lie over them, those too
+      uint64_t* other = j == 0 ? &q_ready[two ? g : 0] : C::APART ? &s_free[g] : &o_done[g];
       if (!warp_wait2(&full[st], (s / C::STAGES) & 1, other, j ? (j - 1) & 1 : 0, a.status)) return false;
       dcu::fence_after();
-      if (lane == 0) {
-        const uint64_t k = dk + st * (C::TILE >> 4), q = dq + (two ? g : 0) * (C::TILE >> 4);
+      const uint64_t k = dk + st * (C::TILE >> 4), q = dq + (two ? g : 0) * (C::TILE >> 4);
+      if (dcu::elect()) {
 #pragma unroll
         for (int kk = 0; kk < 4 * NP; kk++) {
           const uint32_t off = ((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4;
-          dcu::mma_ss(tmem + g * KEYS, q + off, k + off, id_s, kk > 0);
+          dcu::mma_ss(tmem + C::s_col(g), q + off, k + off, id_s, kk > 0);
         }
         dcu::commit(&s_full[g]);
-        if (!two || g == 1) dcu::commit(&empty[st]);
+        if (!two || g) dcu::commit(&empty[st]);
       }
       __syncwarp();
       return true;
@@ -223,21 +236,29 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     for (int j = 0; j < count0 && ok; j++) {
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        if (!ok || j >= (g ? count1 : count0)) continue;
+        const int count = g ? count1 : count0;
+        if (!ok || j >= count) continue;
+        if (C::APART && j + 1 < count) ok = scores(g, j + 1);
         const int s = place_v(two ? j : g + 2 * j), st = s % C::STAGES;
-        ok = warp_wait2(&p_ready[g], j & 1, &full[st], (s / C::STAGES) & 1, a.status);
-        if (!ok) break;
-        dcu::fence_after();
-        if (lane == 0) {
-          const uint64_t v = dv + st * (C::TILE >> 4);
+        const uint64_t v = dv + st * (C::TILE >> 4);
 #pragma unroll
-          for (int kk = 0; kk < KEYS / 16; kk++)
-            dcu::mma_ts(tmem + T_O + g * 128, tmem + g * KEYS + kk * 8, v + (kk * 16 * 128 >> 4), id_o, j > 0 || kk > 0);
-          dcu::commit(&o_done[g]);
-          if (!two || g == 1) dcu::commit(&empty[st]);
+        for (int half = 0; half < 2; half++) {
+          ok = ok && (half ? warp_wait(&p_ready[2 * g + 1], j & 1, a.status)
+                           : warp_wait2(&p_ready[2 * g], j & 1, &full[st], (s / C::STAGES) & 1, a.status));
+          if (!ok) break;
+          dcu::fence_after();
+          if (dcu::elect()) {
+#pragma unroll
+            for (int kk = 4 * half; kk < 4 * half + 4; kk++)
+              dcu::mma_ts(tmem + C::o_col(g), tmem + C::p_col(g) + kk * 8, v + (kk * 16 * 128 >> 4), id_o, j > 0 || kk > 0);
+            if (half) {
+              dcu::commit(&o_done[g]);
+              if (!two || g) dcu::commit(&empty[st]);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (j + 1 < (g ? count1 : count0)) ok = scores(g, j + 1);
+        if (!C::APART && ok && j + 1 < count) ok = scores(g, j + 1);
       }
     }
   } else {
@@ -265,8 +286,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
       if (lane == 0) dcp::mbar_arrive(&q_ready[g]);
     }
     // ---- softmax: this thread's query row is TMEM lane quarter * 32 + lane
-    const uint32_t s_at = tmem + ((uint32_t)(quarter * 32) << 16) + g * KEYS;
-    const uint32_t o_at = tmem + ((uint32_t)(quarter * 32) << 16) + T_O + g * 128;
+    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_at = lane_at + C::s_col(g), o_at = lane_at + C::o_col(g), p_at = lane_at + C::p_col(g);
     const bool used = quarter * 32 < nrows;  // (a warp without rows only keeps the barriers going)
     const int count = g ? count1 : count0;
     float mx = -INFINITY, l = 0.0f;  // the maximum in use (scores before c), the sum
@@ -274,13 +295,21 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     for (int j = 0; j < count; j++) {
       if (!warp_wait(&s_full[g], j & 1, a.status)) { ok = false; break; }
       dcu::fence_after();
+      uint32_t s[4][32];
       if (used) {
-        uint32_t s[4][32];
 #pragma unroll
         for (int x = 0; x < 4; x++) dcu::ld32(s_at + x * 32, s[x]);
 #pragma unroll
         for (int x = 0; x < 4; x++) dcu::wait_ld(s[x]);
-        const int nv = k1 - k0 - (two ? j : g + 2 * j) * KEYS;  // keys of the tile
+      }
+      if (C::APART) {
+        dcu::fence_before();
+        __syncwarp();
+        if (lane == 0) dcp::mbar_arrive(&s_free[g]);
+      }
+      const int nv = k1 - k0 - (two ? j : g + 2 * j) * KEYS;  // keys of the tile
+      F2 c2 = dcu::f2(a.c, a.c), b2 = c2, sum[2] = {dcu::f2(0, 0), dcu::f2(0, 0)};
+      if (used) {
         if (nv < KEYS) {
 #pragma unroll
           for (int x = 0; x < 4; x++)
@@ -288,23 +317,21 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
             for (int y = 0; y < 32; y++)
               if (x * 32 + y >= nv) s[x][y] = __float_as_uint(-INFINITY);
         }
-        float top8[8];
+        float m4[4];
 #pragma unroll
-        for (int y = 0; y < 8; y++) top8[y] = fmaxf(__uint_as_float(s[0][y]), __uint_as_float(s[1][y]));
+        for (int x = 0; x < 4; x++) m4[x] = fmaxf(__uint_as_float(s[x][0]), __uint_as_float(s[x][1]));
 #pragma unroll
-        for (int y = 0; y < 8; y++) top8[y] = fmaxf(top8[y], fmaxf(__uint_as_float(s[2][y]), __uint_as_float(s[3][y])));
+        for (int y = 2; y < 32; y += 2)
 #pragma unroll
-        for (int y = 8; y < 32; y++) {
-          top8[y & 7] = fmaxf(top8[y & 7], fmaxf(__uint_as_float(s[0][y]), __uint_as_float(s[1][y])));
-          top8[y & 7] = fmaxf(top8[y & 7], fmaxf(__uint_as_float(s[2][y]), __uint_as_float(s[3][y])));
-        }
-        const float top = fmaxf(fmaxf(fmaxf(top8[0], top8[1]), fmaxf(top8[2], top8[3])),
-                                fmaxf(fmaxf(top8[4], top8[5]), fmaxf(top8[6], top8[7])));
+          for (int x = 0; x < 4; x++) m4[x] = dcu::max3(m4[x], __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
+        const float top = fmaxf(dcu::max3(m4[0], m4[1], m4[2]), m4[3]);
         if (j == 0) {
           mx = top;
         } else if (__any_sync(~0u, top > mx && !((top - mx) * a.c <= RAISE))) {
-          // O *= 2^(c (old - new)).  (These scores were issued behind the end of
-          // the product of the tile before: O holds it, and nothing writes O.)
+          // O *= 2^(c (old - new)), once it holds the product of the tile before
+          // (the next product needs these probabilities)
+          if (C::APART && !warp_wait(&o_done[g], (j - 1) & 1, a.status)) { ok = false; break; }
+          dcu::fence_after();
           const float up = fmaxf(mx, top);
           const float f = mx == -INFINITY ? 0.0f : mx == up ? 1.0f : dcu::ex2((mx - up) * a.c);
           mx = up;
@@ -321,31 +348,46 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           dcu::wait_st();
         }
         const float base = mx == -INFINITY ? 0.0f : mx * a.c;
-        const F2 c2 = dcu::f2(a.c, a.c), b2 = dcu::f2(-base, -base);
-        F2 sum[2] = {dcu::f2(0, 0), dcu::f2(0, 0)};
-#pragma unroll
-        for (int x = 0; x < 4; x += 2) {
-          uint32_t p[32];
-#pragma unroll
-          for (int y = 0; y < 32; y++) {
-            // (the sum keeps the unrounded values: lse is exact to f32; P is
-            // rounded to the type of the products' operands, half a step each)
-            const uint32_t(&u)[32] = s[x + y / 16];
-            const int k = (y % 16) * 2;
-            const float2 e = dcu::split(dcu::fma2(dcu::f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, b2));
-            const float e0 = dcu::ex2(e.x), e1 = dcu::ex2(e.y);
-            sum[y & 1] = dcu::add2(sum[y & 1], dcu::f2(e0, e1));
-            p[y] = pack2<BF16>(e0, e1);
-          }
-          dcu::st32(s_at + x * 16, p);
-        }
-        const float2 both = dcu::split(dcu::add2(sum[0], sum[1]));
-        l += both.x + both.y;
-        dcu::wait_st();
+        b2 = dcu::f2(-base, -base);
       }
-      dcu::fence_before();
-      __syncwarp();
-      if (lane == 0) dcp::mbar_arrive(&p_ready[g]);
+      bool met = true;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        // (a warp without rows waits too: its arrival belongs to this tile's phase)
+        if (C::APART && !used && half == 0 && j > 0) met = warp_wait(&o_done[g], (j - 1) & 1, a.status);
+        if (used) {
+#pragma unroll
+          for (int x = 2 * half; x < 2 * half + 2; x++) {
+            uint32_t p[16];
+#pragma unroll
+            for (int y = 0; y < 16; y++) {
+              // (the sum keeps the unrounded values: lse is exact to f32; P is
+              // rounded to the type of the products' operands, half a step each)
+              F2 e = dcu::fma2(dcu::f2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), c2, b2);
+              if (y % FMA_EVERY == FMA_EVERY - 1) {
+                e = dcu::ex2_fma(e);
+              } else {
+                const float2 v = dcu::split(e);
+                e = dcu::f2(dcu::ex2(v.x), dcu::ex2(v.y));
+              }
+              sum[y & 1] = dcu::add2(sum[y & 1], e);
+              const float2 v = dcu::split(e);
+              p[y] = pack2<BF16>(v.x, v.y);
+            }
+            // (beside the scores: where the product of the tile before has read the ones there)
+            if (C::APART && x == 0 && j > 0) met = warp_wait(&o_done[g], (j - 1) & 1, a.status);
+            dcu::fence_after();
+            dcu::st16(p_at + x * 16, p);
+          }
+          dcu::wait_st();
+        }
+        dcu::fence_before();
+        __syncwarp();
+        if (lane == 0) dcp::mbar_arrive(&p_ready[2 * g + half]);
+      }
+      const float2 both = dcu::split(dcu::add2(sum[0], sum[1]));
+      l += both.x + both.y;
+      if (!met) { ok = false; break; }
     }
     if (used) {
       const int row = quarter * 32 + lane;

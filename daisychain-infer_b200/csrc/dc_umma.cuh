@@ -56,6 +56,21 @@ __device__ __forceinline__ constexpr uint32_t idesc(bool bf16, int n, bool b_mn)
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
          ((128u >> 4) << 24);
 }
+// True in one lane of a converged warp, for `if (elect())` around products and
+// commits: the compiler knows this form, and their operands stay in uniform
+// registers (eight products issue in 100 to 165 cycles; under `if (lane == 0)` in
+// 385, which then bounded the softmax kernels).
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+// A value that is the same in all lanes, as one the compiler knows to be.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(~0u, v, 0); }
 // D (TMEM) (+)= A (shared) x B (shared)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(
@@ -74,6 +89,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
+// One arrival on `bar` once the products that this lane issued so far are complete.
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    dcp::smem_u32(bar))
@@ -166,6 +182,35 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   F2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of both halves on the multiply-add pipe, for where the exponential unit
+// (16 a cycle and SM) is what a kernel waits for: x = n + f with n whole and |f|
+// <= 1/2 (n by adding 1.5 x 2^23), 2^f by its best polynomial of degree five (7.5e-8
+// relative, from a Remez iteration; 2.1e-7 with the f32 roundings, as the unit's
+// own 2.4e-7), 2^n from its exponent field.  0 from x = -126.5 down, inf from 127.5
+// up, NaN for NaN.
+__device__ __forceinline__ F2 ex2_fma(F2 x) {
+  float2 v = split(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(128.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(128.0f));
+  const F2 y = f2(v.x, v.y), t = add2(y, f2(12582912.0f, 12582912.0f));
+  const F2 f = fma2(add2(t, f2(-12582912.0f, -12582912.0f)), f2(-1.0f, -1.0f), y);
+  F2 p = fma2(f, f2(0.0013276472454890609f, 0.0013276472454890609f), f2(0.009675540961325169f, 0.009675540961325169f));
+  p = fma2(p, f, f2(0.05550713092088699f, 0.05550713092088699f));
+  p = fma2(p, f, f2(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, f2(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, f, f2(1.0000001192092896f, 1.0000001192092896f));
+  const float2 w = split(t);
+  return mul2(p, f2(__int_as_float((__float_as_int(w.x) << 23) + 0x3f800000),
+                    __int_as_float((__float_as_int(w.y) << 23) + 0x3f800000)));
 }
 
 // A tensor map over `rank` dimensions of a 16-bit tensor; strides[i] (bytes)

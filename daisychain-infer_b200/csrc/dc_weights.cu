@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint64_t* kept_full = s_free + 2;
   uint32_t* slot = (uint32_t*)(kept_full + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int split = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
   const int h = bg % a.kv_heads, b = bg / a.kv_heads;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   dcu::fence_before();
   __syncthreads();
   dcu::fence_after();
-  const uint32_t tmem = *slot;
+  const uint32_t tmem = dcu::uniform(*slot);
   // (only now: a dependent that takes TMEM before its own wait must not take
   // what a block of this grid still has to get)
   asm volatile("griddepcontrol.launch_dependents;");
@@ -152,26 +152,30 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
     }
   } else if (warp == 5) {
-    if (lane == 0) {
+    {
       const uint32_t id = dcu::idesc(BF16, 0, false) | ((uint32_t)(a.cols_mma >> 3) << 17);
       const uint32_t kept_at = dcp::smem_u32(kept), ring_at = dcp::smem_u32(ring);
-      bool ok = dcp::mbar_wait(kept_full, 0, a.status);
+      bool ok = __all_sync(~0u, dcp::mbar_wait(kept_full, 0, a.status));
       for (int i = 0; i < n && ok; i++) {
-        if (i >= 2) ok = dcp::mbar_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status);
+        if (i >= 2) ok = __all_sync(~0u, dcp::mbar_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status));
 #pragma unroll
         for (int p = 0; p < NP; p++) {
           const int s = i * NP + p, st = s % STAGES;
-          ok = ok && dcp::mbar_wait(&full[st], (s / STAGES) & 1, a.status);
+          ok = ok && __all_sync(~0u, dcp::mbar_wait(&full[st], (s / STAGES) & 1, a.status));
           if (!ok) break;
           dcu::fence_after();
           const uint32_t keep = kept_at + p * PANEL_BYTES, move = ring_at + st * PANEL_BYTES;
+          const uint64_t dkeep = dcu::desc(keep, 0), dmove = dcu::desc(move, 0);
+          if (dcu::elect()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++)
-            dcu::mma_ss(tmem + (i & 1) * COLS, dcu::desc((KEEP_Q ? move : keep) + kk * 32, 0),
-                        dcu::desc((KEEP_Q ? keep : move) + kk * 32, 0), id, p > 0 || kk > 0);
-          dcu::commit(&empty[st]);
+            for (int kk = 0; kk < 4; kk++)
+              dcu::mma_ss(tmem + (i & 1) * COLS, (KEEP_Q ? dmove : dkeep) + kk * 2, (KEEP_Q ? dkeep : dmove) + kk * 2, id,
+                          p > 0 || kk > 0);
+            dcu::commit(&empty[st]);
+            if (p == NP - 1) dcu::commit(&s_full[i & 1]);
+          }
+          __syncwarp();
         }
-        if (ok) dcu::commit(&s_full[i & 1]);
       }
     }
   } else {
