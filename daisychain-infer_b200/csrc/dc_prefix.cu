@@ -89,8 +89,8 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 
 // ---- the shared prefix ----------------------------------------------------------
 // Two groups of four warps take the softmax of a 128 x 128 tile of scores, a
-// thread a query row (TMEM lane); warp 8 streams 128-key tiles through a ring by
-// TMA, warp 9 issues the products
+// thread a query row (TMEM lane); one more warp streams 128-key tiles through a
+// ring by TMA, another issues the products
 //   S = Q K^T (128 x 128, f32 in TMEM),  O += P V (128 x hd in TMEM)
 // with P rounded to the keys' type.  With two tiles of rows each group has its
 // own and both use each tile of keys; a tile of rows that is left over has a block
@@ -102,15 +102,17 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // Wider ones have P written over S, and the next scores wait for the product.
 // Either way P goes out in two halves, so that the product starts on the first.
 //
-// Per 128 x 128 tile and SM the exponential unit needs 1024 cycles (a quarter less
-// with every fourth pair taken on the multiply-add pipe), the products 500 + 500,
-// shared memory 512 + 256 for their operands and 256 for the copies: with 64-key
-// tiles in two smaller blocks an SM the operands and copies alone took 1536
-// (measured 1975 cycles a tile).
+// Per 128 x 128 tile and SM the exponential unit needs 1024 cycles, the products 500
+// + 500, shared memory 512 + 256 for their operands and 256 for the copies: with
+// 64-key tiles in two smaller blocks an SM the operands and copies alone took 1536.
+// Measured: about 1950 cycles a tile (of a group's turn, half is its softmax, a
+// quarter its products, the rest waits and the issuing warp).
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
-constexpr int FMA_EVERY = 4;  // every fourth pair of exponentials on the multiply-add pipe
-constexpr int SH_THREADS = 320;
+constexpr int SH_THREADS = 384;
+// (the oldest warps: when the softmax's many instructions compete with theirs for
+// a scheduler, theirs go first)
+constexpr int MMA_WARP = 0, TMA_WARP = 1, EXP_WARP = 4;
 
 template <int NP>
 struct Shared {
@@ -121,6 +123,11 @@ struct Shared {
   static constexpr int SMEM = (2 + STAGES) * TILE + 256;
   // TMEM columns of group g: scores, O, probabilities
   static constexpr bool APART = NP == 1;  // probabilities beside the scores
+  // every so many pairs of exponentials one on the multiply-add pipe: 64
+  // sequences over 65536 keys take 114 us with none, 104 with one in eight,
+  // 105 to 110 with one in four; at 64 channels a head none is best (60 against
+  // 64 us)
+  static constexpr int FMA_EVERY = NP == 2 ? 8 : 1 << 20;
   static constexpr uint32_t s_col(int g) { return g * 128; }
   static constexpr uint32_t o_col(int g) { return 256 + g * WIDTH; }
   static constexpr uint32_t p_col(int g) { return APART ? 384 + g * 64 : s_col(g); }
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     }
     dcp::mbar_fence_init();
   }
-  if (warp == 9) dcu::alloc(slot, 512);
+  if (warp == MMA_WARP) dcu::alloc(slot, 512);
   dcu::fence_before();
   __syncthreads();
   dcu::fence_after();
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
   auto place_k = [&](int i) { return two ? 2 * i : i ? 2 * i - 1 : 0; };
   auto place_v = [&](int i) { return two ? 2 * i + 1 : i + 1 < n ? 2 * i + 2 : 2 * n - 1; };
 
-  if (warp == 8) {
+  if (warp == TMA_WARP) {
     if (lane == 0) {
       // ---- copies
       int issued = 0;
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
         for (int s = max(0, issued - C::STAGES); s < issued; s++)
           dcp::mbar_wait(&full[s % C::STAGES], (s / C::STAGES) & 1, a.status);
     }
-  } else if (warp == 9) {
+  } else if (warp == MMA_WARP) {
     // ---- products, of the groups by turns: that keeps their softmaxes half a
     // tile apart (with a warp for each group they fell into step, and waited
     // for the tensor pipe and the exponential unit at the same times)
@@ -261,8 +268,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
         if (!C::APART && ok && j + 1 < count) ok = scores(g, j + 1);
       }
     }
-  } else {
-    const int g = warp >> 2, quarter = warp & 3;  // group, TMEM lanes
+  } else if (warp >= EXP_WARP) {
+    const int g = (warp - EXP_WARP) >> 2, quarter = warp & 3;  // group, TMEM lanes
     const int m = 2 * pair + (two ? g : 0);
     const int nrows = min(ROWS, a.pre_rows - m * ROWS);
     // ---- Q into shared memory: each lane its own row's place, then rows by
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
               // (the sum keeps the unrounded values: lse is exact to f32; P is
               // rounded to the type of the products' operands, half a step each)
               F2 e = dcu::fma2(dcu::f2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), c2, b2);
-              if (y % FMA_EVERY == FMA_EVERY - 1) {
+              if (y % C::FMA_EVERY == C::FMA_EVERY - 1) {
                 e = dcu::ex2_fma(e);
               } else {
                 const float2 v = dcu::split(e);
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     dcu::fence_before();
   }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == MMA_WARP) {
     dcu::fence_after();
     dcu::dealloc(tmem, 512);
   }
