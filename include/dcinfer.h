@@ -261,9 +261,9 @@ int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* a, void* ws, size
  * for j < lens[b] (clamped to [0, cache]); the rest of acc is left as it is.
  * causal = 1: row r sees tokens j < lens[b] - (rows - 1 - r), as above; 0: all
  * rows see all tokens (a shared prefix: batch 1, the batch's rows as rows).
- * decay = 0 overwrites without reading acc; a row of lse -inf adds nothing.  The
- * sum's order is fixed: equal inputs give equal bits.  Types and alignment as
- * above; heads / kv_heads <= 128. */
+ * decay (rounded to f32) = 0 overwrites without reading acc; a row of lse -inf
+ * adds nothing.  The sum's order is fixed: equal inputs give equal bits.  Types
+ * and alignment as above; heads / kv_heads <= 128. */
 typedef struct dc_cache_weight {
   const void *q, *k;
   const int32_t* lens;
