@@ -8,16 +8,19 @@
 // one key against all rows and adds its exponentials in a register: no
 // exchange, no atomics, one order of summation.
 //
-// Few rows (one column tile): a block keeps Q and streams its share of the
-// cache's keys; HBM-bound, each key is read once.  Many rows: a block keeps 128
-// keys and streams Q tiles (out of L2) past them; bound by the exponential unit,
-// 16 a cycle and SM: 128 x 128 of them take 1024 cycles, their products 512.
-// Two blocks share an SM, and the scores are double-buffered in TMEM, so copies
-// and products run under the exponentials.
+// k_weights_few, up to 128 columns: a block keeps Q in shared memory and streams
+// its share of the cache's keys (16 KB panels through a ring by TMA), two blocks an
+// SM, scores double-buffered in TMEM.  HBM-bound: each key is read once.
 //
-// Warps 0-3 own a TMEM lane (key) per thread, warp 4 copies 64-element panels
-// (16 KB) into a ring by TMA, warp 5 issues the products.  Every wait is
-// bounded; a block whose wait gives up ends, and dc_sync reports it.
+// k_weights_many: a block keeps 256 keys in TMEM, as the first operand, for two
+// groups of four warps, and streams Q tiles (out of L2) past both.  Bound by the
+// exponential unit, 16 a cycle and SM: 128 x 128 of them take 1024 cycles, their
+// products 500 and their operands 256 of shared memory's (with the keys in shared
+// memory too, in two blocks an SM, the operands and copies took 768 and the whole
+// 1980 a tile).
+//
+// One warp copies, one issues the products.  Every wait is bounded; a block whose
+// wait gives up ends, and dc_sync reports it.
 #include <algorithm>
 
 #include "dc_cache.cuh"
@@ -30,46 +33,99 @@ using dcu::F2;
 
 constexpr int KEYS = 128;   // keys of a tile: the MMA's M
 constexpr int COLS = 128;   // query rows of a tile: its N
-constexpr int THREADS = 192;
+constexpr int FEW_THREADS = 192;
+constexpr int MANY_EVERY = 4;
 constexpr int PANEL_BYTES = 128 * 128;
-constexpr uint32_t TMEM_COLS = 256;  // two buffers of COLS scores
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Two blocks an SM hold at most 113 KB each: beside two panels of the kept tile
-// and the scales, five ring stages or (two buffers of scales) four.
-template <int NP, bool KEEP_Q>
-struct Cfg {
-  static constexpr int STAGES = KEEP_Q || NP == 1 ? 5 : 4;
-  static constexpr int SCALES = KEEP_Q ? 1 : 2;
-  static constexpr int SMEM = (NP + STAGES) * PANEL_BYTES + SCALES * COLS * 4 + 128;
-};
+constexpr int STAGES = 5;  // two blocks an SM hold at most 113 KB each
+template <int NP>
+constexpr int FEW_SMEM = (NP + STAGES) * PANEL_BYTES + COLS * 4 + 128;
 
 struct CwArgs {
+  const void* k;
   const int32_t* lens;
   const float* lse;
   float* acc;
-  int64_t acc_seq, acc_head;
+  int64_t k_seq, k_tok, k_head, acc_seq, acc_head;
   float c, decay;
-  int rows, heads, kv_heads, group, cache, causal;
+  int rows, heads, kv_heads, group, hd, cache, causal;
   int tile_rows, tile_cols, col_tiles;  // rows and columns (rows x group) of a Q tile
   int chunk, splits;                    // keys of a block, blocks of a head
   int cols_mma;                         // the products' N
   int* status;
 };
 
-// KEEP_Q: the block keeps its one Q tile and streams keys; otherwise it keeps
-// its one key tile and streams Q tiles.
-template <int NP, bool BF16, bool KEEP_Q>
-__global__ void __launch_bounds__(THREADS, 2)
-    k_cache_weights(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
-                    const __grid_constant__ CwArgs a) {
-  using C = Cfg<NP, KEEP_Q>;
-  constexpr int STAGES = C::STAGES;
+// The exponentials of 32 columns c0.. of a tile (scores x, scales L) added to
+// `part`: those from column `from` up to `cols`.  Every `every`-th pair is taken on the
+// multiply-add pipe.
+template <int EVERY>
+__device__ __forceinline__ void add_columns(F2 (&part)[4], const uint32_t (&x)[32], const float* L, float c, int c0,
+                                            int from, int cols, bool late) {
+  if (late || c0 + 32 > cols) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+      const float e = dcu::ex2(fmaf(__uint_as_float(x[j]), c, L[c0 + j]));
+      part[j & 3] = dcu::add2(part[j & 3], dcu::f2(c0 + j < from || c0 + j >= cols ? 0.0f : e, 0.0f));
+    }
+    return;
+  }
+  const F2 c2 = dcu::f2(c, c);
+  const float4* l4 = reinterpret_cast<const float4*>(L + c0);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float4 l = l4[j];
+    const F2 lp[2] = {dcu::f2(l.x, l.y), dcu::f2(l.z, l.w)};
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      const int k = 4 * j + 2 * y;
+      F2 e = dcu::fma2(dcu::f2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), c2, lp[y]);
+      if ((2 * j + y) % EVERY == EVERY - 1) {
+        e = dcu::ex2_fma(e);
+      } else {
+        const float2 v = dcu::split(e);
+        e = dcu::f2(dcu::ex2(v.x), dcu::ex2(v.y));
+      }
+      part[(2 * j + y) & 3] = dcu::add2(part[(2 * j + y) & 3], e);
+    }
+  }
+}
+__device__ __forceinline__ float sum_of(const F2 (&part)[4]) {
+  const float2 v = dcu::split(dcu::add2(dcu::add2(part[0], part[1]), dcu::add2(part[2], part[3])));
+  return v.x + v.y;
+}
+// lse of column col of Q tile t (+inf: no row), and what is added to a column's
+// exponents: -lse * log2 e, -inf where nothing is to be summed.
+__device__ __forceinline__ float lse_of(const CwArgs& a, int64_t lse_at, int t, int col) {
+  const int row = t * a.tile_rows + col / a.group;
+  return col < a.tile_cols && row < a.rows ? a.lse[lse_at + (int64_t)row * a.heads + col % a.group] : INFINITY;
+}
+__device__ __forceinline__ float scale_of(float lse) { return lse == -INFINITY ? -INFINITY : -lse * LOG2E; }
+__device__ __forceinline__ void put(const CwArgs& a, int b, int h, int key, float sum) {
+  float* at = a.acc + b * a.acc_seq + h * a.acc_head + key;
+  *at = a.decay == 0.0f ? sum : fmaf(a.decay, *at, sum);
+}
+// Panel rows that no Q copy writes (128 is no multiple of the group): zero, so
+// that their scores are 0 and not what the memory held.
+__device__ __forceinline__ void zero_rows(uint8_t* panels, int count, int tile_cols, int threads) {
+  if (tile_cols >= COLS) return;
+  const int per = (COLS - tile_cols) * 8;
+  for (int i = threadIdx.x; i < per * count; i += threads) {
+    const int p = i / per, rest = i - p * per;
+    *reinterpret_cast<uint4*>(panels + p * PANEL_BYTES + tile_cols * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+template <int NP, bool BF16>
+__global__ void __launch_bounds__(FEW_THREADS, 2)
+    k_weights_few(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ CwArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* kept = smem;
   uint8_t* ring = smem + NP * PANEL_BYTES;
-  float* scales = (float*)(ring + STAGES * PANEL_BYTES);  // -lse * log2 e of a tile's columns; -inf where nothing is added
-  uint64_t* full = (uint64_t*)(scales + C::SCALES * COLS);
+  float* L = (float*)(ring + STAGES * PANEL_BYTES);  // the columns' scales
+  uint64_t* full = (uint64_t*)(L + COLS);
   uint64_t* empty = full + STAGES;
   uint64_t* s_full = empty + STAGES;  // [2] scores of a buffer are in TMEM
   uint64_t* s_free = s_full + 2;      // [2] and have been read
@@ -83,11 +139,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int len = max(0, min(a.lens[b], a.cache));
   const int k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
   if (k1 <= k0) return;
-  // (key tile, Q tile) pairs in turn: KEEP_Q walks the keys, else the Q tiles,
-  // from the first that holds a row which sees the block's first key
-  const int see0 = a.causal ? max(0, k0 - len + a.rows) : 0;  // first row that sees key k0
-  const int t0 = KEEP_Q ? 0 : see0 / a.tile_rows;
-  const int n = KEEP_Q ? (k1 - k0 + KEYS - 1) / KEYS : a.col_tiles - t0;
+  const int n = (k1 - k0 + KEYS - 1) / KEYS;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
@@ -101,18 +153,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     dcp::mbar_init(kept_full, 1);
     dcp::mbar_fence_init();
   }
-  if (warp == 5) dcu::alloc(slot, TMEM_COLS);
-  // panel rows that no Q copy writes (128 is no multiple of the group): zero,
-  // so that their scores are 0 and not what the memory held
-  if (a.tile_cols < COLS) {
-    uint8_t* at = KEEP_Q ? kept : ring;
-    const int per = (COLS - a.tile_cols) * 8, panels = KEEP_Q ? NP : STAGES;
-    for (int i = threadIdx.x; i < per * panels; i += THREADS) {
-      const int p = i / per, rest = i - p * per;
-      *reinterpret_cast<uint4*>(at + p * PANEL_BYTES + a.tile_cols * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
+  if (warp == 5) dcu::alloc(slot, 2 * COLS);
+  zero_rows(kept, NP, a.tile_cols, FEW_THREADS);
+  if (threadIdx.x < COLS) L[threadIdx.x] = scale_of(lse_of(a, (int64_t)b * a.rows * a.heads + h * a.group, 0, threadIdx.x));
   dcu::fence_before();
   __syncthreads();
   dcu::fence_after();
@@ -121,28 +164,17 @@ __global__ void __launch_bounds__(THREADS, 2)
   // what a block of this grid still has to get)
   asm volatile("griddepcontrol.launch_dependents;");
 
-  const int q_bytes = a.tile_cols * 128;
   if (warp == 4) {
     if (lane == 0) {
-      const int kept_bytes = KEEP_Q ? q_bytes : PANEL_BYTES, ring_bytes = KEEP_Q ? PANEL_BYTES : q_bytes;
-      dcp::mbar_expect_tx(kept_full, NP * kept_bytes);
+      dcp::mbar_expect_tx(kept_full, NP * a.tile_cols * 128);
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        if (KEEP_Q)
-          dcu::tma_load_5d(kept + p * PANEL_BYTES, &map_q, p * 64, 0, h, 0, b, kept_full);
-        else
-          dcu::tma_load_4d(kept + p * PANEL_BYTES, &map_k, p * 64, h, k0, b, kept_full);
-      }
+      for (int p = 0; p < NP; p++) dcu::tma_load_5d(kept + p * PANEL_BYTES, &map_q, p * 64, 0, h, 0, b, kept_full);
       int issued = 0;
       for (int s = 0; s < n * NP; s++, issued++) {
         const int st = s % STAGES, i = s / NP, p = s - i * NP;
         if (s >= STAGES && !dcp::mbar_wait(&empty[st], ((s / STAGES) & 1) ^ 1, a.status)) break;
-        dcp::mbar_expect_tx(&full[st], ring_bytes);
-        uint8_t* dst = ring + st * PANEL_BYTES;
-        if (KEEP_Q)
-          dcu::tma_load_4d(dst, &map_k, p * 64, h, k0 + i * KEYS, b, &full[st]);
-        else
-          dcu::tma_load_5d(dst, &map_q, p * 64, 0, h, (t0 + i) * a.tile_rows, b, &full[st]);
+        dcp::mbar_expect_tx(&full[st], PANEL_BYTES);
+        dcu::tma_load_4d(ring + st * PANEL_BYTES, &map_k, p * 64, h, k0 + i * KEYS, b, &full[st]);
       }
       if (issued < n * NP) {
         // (given up: what is in flight lands before the block's memory goes away)
@@ -152,122 +184,231 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
     }
   } else if (warp == 5) {
-    {
-      const uint32_t id = dcu::idesc(BF16, 0, false) | ((uint32_t)(a.cols_mma >> 3) << 17);
-      const uint32_t kept_at = dcp::smem_u32(kept), ring_at = dcp::smem_u32(ring);
-      bool ok = __all_sync(~0u, dcp::mbar_wait(kept_full, 0, a.status));
-      for (int i = 0; i < n && ok; i++) {
-        if (i >= 2) ok = __all_sync(~0u, dcp::mbar_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status));
+    const uint32_t id = dcu::idesc(BF16, 0, false) | ((uint32_t)(a.cols_mma >> 3) << 17);
+    const uint64_t dq = dcu::desc(dcp::smem_u32(kept), 0), dk = dcu::desc(dcp::smem_u32(ring), 0);
+    bool ok = __all_sync(~0u, dcp::mbar_wait(kept_full, 0, a.status));
+    for (int i = 0; i < n && ok; i++) {
+      if (i >= 2) ok = __all_sync(~0u, dcp::mbar_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status));
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-          const int s = i * NP + p, st = s % STAGES;
-          ok = ok && __all_sync(~0u, dcp::mbar_wait(&full[st], (s / STAGES) & 1, a.status));
-          if (!ok) break;
-          dcu::fence_after();
-          const uint32_t keep = kept_at + p * PANEL_BYTES, move = ring_at + st * PANEL_BYTES;
-          const uint64_t dkeep = dcu::desc(keep, 0), dmove = dcu::desc(move, 0);
-          if (dcu::elect()) {
+      for (int p = 0; p < NP; p++) {
+        const int s = i * NP + p, st = s % STAGES;
+        ok = ok && __all_sync(~0u, dcp::mbar_wait(&full[st], (s / STAGES) & 1, a.status));
+        if (!ok) break;
+        dcu::fence_after();
+        if (dcu::elect()) {
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              dcu::mma_ss(tmem + (i & 1) * COLS, (KEEP_Q ? dmove : dkeep) + kk * 2, (KEEP_Q ? dkeep : dmove) + kk * 2, id,
-                          p > 0 || kk > 0);
-            dcu::commit(&empty[st]);
-            if (p == NP - 1) dcu::commit(&s_full[i & 1]);
-          }
-          __syncwarp();
+          for (int kk = 0; kk < 4; kk++)
+            dcu::mma_ss(tmem + (i & 1) * COLS, dk + st * (PANEL_BYTES >> 4) + kk * 2, dq + p * (PANEL_BYTES >> 4) + kk * 2,
+                        id, p > 0 || kk > 0);
+          dcu::commit(&empty[st]);
+          if (p == NP - 1) dcu::commit(&s_full[i & 1]);
         }
+        __syncwarp();
       }
     }
   } else {
     const uint32_t lane_at = tmem + ((uint32_t)(warp * 32) << 16);
-    const int64_t lse_at = (int64_t)b * a.rows * a.heads + h * a.group;
-    // column `threadIdx.x` of Q tile t
-    auto column = [&](int t) {
-      const int col = threadIdx.x, row = t * a.tile_rows + col / a.group;
-      float v = -INFINITY;
-      if (col < a.tile_cols && row < a.rows) {
-        v = -a.lse[lse_at + (int64_t)row * a.heads + col % a.group] * LOG2E;
-        if (v == INFINITY) v = -INFINITY;
-      }
-      return v;
-    };
-    float next = column(t0);
-    float sum = 0.0f;
-    bool ok = true;  // (a warp whose wait gave up stays in the loop: the others count on it at the barrier)
+    const int cols = a.tile_cols;
     for (int i = 0; i < n; i++) {
-      float* L = scales + (KEEP_Q ? 0 : (i & 1) * COLS);
-      if (!KEEP_Q || i == 0) {
-        L[threadIdx.x] = next;
-        if (!KEEP_Q && i + 1 < n) next = column(t0 + i + 1);
-        // (one barrier a tile: who passes it has read the buffer of two tiles ago)
-        dcp::named_sync(1, 128);
-      }
-      ok = ok && __all_sync(~0u, dcp::mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.status));
-      if (!ok) continue;
+      if (!__all_sync(~0u, dcp::mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.status))) break;
       dcu::fence_after();
-      const int key = (KEEP_Q ? k0 + i * KEYS : k0) + warp * 32 + lane;
-      const int first_row = KEEP_Q ? 0 : (t0 + i) * a.tile_rows;
-      // columns of this tile that see the key
-      const int from = a.causal ? max(0, (key - len + a.rows - first_row)) * a.group : 0;
-      const int cols = min(a.tile_cols, (a.rows - first_row) * a.group);
+      const int key = k0 + i * KEYS + warp * 32 + lane;
+      const int from = a.causal ? max(0, key - len + a.rows) * a.group : 0;  // columns that see the key
       const bool late = __any_sync(~0u, from > 0);
-      if (KEEP_Q) sum = 0.0f;
-      const F2 c2 = dcu::f2(a.c, a.c);
       F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
-      uint32_t s[2][32];
-      // columns c0 .. c0 + 31, and the next ones' load meanwhile
-      auto add = [&](uint32_t (&x)[32], uint32_t (&next)[32], int c0) {
-        dcu::wait_ld(x);
-        if (c0 + 32 < cols) dcu::ld32(lane_at + (i & 1) * COLS + c0 + 32, next);
-        const float4* l4 = reinterpret_cast<const float4*>(L + c0);
-        if (late || c0 + 32 > cols) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) {
-            const float e = dcu::ex2(fmaf(__uint_as_float(x[j]), a.c, L[c0 + j]));
-            part[j & 3] = dcu::add2(part[j & 3], dcu::f2(c0 + j < from || c0 + j >= cols ? 0.0f : e, 0.0f));
-          }
-          return;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float4 l = l4[j];
-          const float2 t0 = dcu::split(
-              dcu::fma2(dcu::f2(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), c2, dcu::f2(l.x, l.y)));
-          const float2 t1 = dcu::split(
-              dcu::fma2(dcu::f2(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), c2, dcu::f2(l.z, l.w)));
-          part[(2 * j) & 3] = dcu::add2(part[(2 * j) & 3], dcu::f2(dcu::ex2(t0.x), dcu::ex2(t0.y)));
-          part[(2 * j + 1) & 3] = dcu::add2(part[(2 * j + 1) & 3], dcu::f2(dcu::ex2(t1.x), dcu::ex2(t1.y)));
-        }
-      };
-      dcu::ld32(lane_at + (i & 1) * COLS, s[0]);
 #pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 64) {
-        add(s[0], s[1], c0);
-        if (c0 + 32 < cols) add(s[1], s[0], c0 + 32);
+      for (int c0 = 0; c0 < cols; c0 += 32) {
+        uint32_t x[32];
+        dcu::ld32(lane_at + (i & 1) * COLS + c0, x);
+        dcu::wait_ld(x);
+        add_columns<1 << 20>(part, x, L, a.c, c0, from, cols, late);
       }
-      const float2 got = dcu::split(dcu::add2(dcu::add2(part[0], part[1]), dcu::add2(part[2], part[3])));
-      sum += got.x + got.y;
       dcu::fence_before();
       __syncwarp();
       if (lane == 0) dcp::mbar_arrive(&s_free[i & 1]);
-      if ((KEEP_Q || i == n - 1) && key < k1) {
-        float* at = a.acc + b * a.acc_seq + h * a.acc_head + key;
-        *at = a.decay == 0.0f ? sum : fmaf(a.decay, *at, sum);
-      }
+      if (key < k1) put(a, b, h, key, sum_of(part));
     }
   }
   __syncthreads();
   if (warp == 5) {
     dcu::fence_after();
-    dcu::dealloc(tmem, TMEM_COLS);
+    dcu::dealloc(tmem, 2 * COLS);
+  }
+}
+
+// Blocks of 2 x 128 keys against all Q tiles.  TMEM columns of group g: its keys
+// (64 x 32 bits a lane), its scores.
+constexpr int MANY_THREADS = 384, MMA_WARP = 0, TMA_WARP = 1, EXP_WARP = 4;
+constexpr uint32_t k_col(int g) { return g * 64; }
+constexpr uint32_t s_col(int g) { return 128 + g * COLS; }
+template <int NP>
+struct Many {
+  static constexpr int TILE = NP * PANEL_BYTES;
+  static constexpr int STAGES = NP == 2 ? 6 : 8;
+  static constexpr int SMEM = STAGES * TILE + 2 * 2 * COLS * 4 + 256;
+};
+
+template <int NP, bool BF16>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+    k_weights_many(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CwArgs a) {
+  using C = Many<NP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem;
+  float* scales = (float*)(ring + C::STAGES * C::TILE);  // [2 groups][2 tiles][COLS]
+  uint64_t* full = (uint64_t*)(scales + 4 * COLS);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* s_full = empty + C::STAGES;  // [2] a group's scores are in TMEM
+  uint64_t* s_free = s_full + 2;         // [2] and have been read (first: its keys are there)
+  uint32_t* slot = (uint32_t*)(s_free + 2);
+
+  const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int split = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
+  const int h = bg % a.kv_heads, b = bg / a.kv_heads;
+  const int len = max(0, min(a.lens[b], a.cache));
+  const int k0 = split * 2 * KEYS;
+  if (len <= k0) return;
+  const int groups = len > k0 + KEYS ? 2 : 1;
+  // Q tiles from the first that holds a row which sees the block's first key
+  const int t0 = a.causal ? max(0, k0 - len + a.rows) / a.tile_rows : 0, n = a.col_tiles - t0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; i++) {
+      dcp::mbar_init(&full[i], 1);
+      dcp::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      dcp::mbar_init(&s_full[i], 1);
+      dcp::mbar_init(&s_free[i], 4);
+    }
+    dcp::mbar_fence_init();
+  }
+  if (warp == MMA_WARP) dcu::alloc(slot, 512);
+  zero_rows(ring, C::STAGES * NP, a.tile_cols, MANY_THREADS);
+  dcu::fence_before();
+  __syncthreads();
+  dcu::fence_after();
+  const uint32_t tmem = dcu::uniform(*slot);
+  // (only now: see k_weights_few)
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  if (warp == TMA_WARP) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < n; i++, issued++) {
+        const int st = i % C::STAGES;
+        if (i >= C::STAGES && !dcp::mbar_wait(&empty[st], ((i / C::STAGES) & 1) ^ 1, a.status)) break;
+        dcp::mbar_expect_tx(&full[st], NP * a.tile_cols * 128);
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+          dcu::tma_load_5d(ring + st * C::TILE + p * PANEL_BYTES, &map_q, p * 64, 0, h, (t0 + i) * a.tile_rows, b, &full[st]);
+      }
+      // (given up: what is in flight lands before the block's memory goes away)
+      if (issued < n)
+        for (int i = max(0, issued - C::STAGES); i < issued; i++)
+          dcp::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, a.status);
+    }
+  } else if (warp == MMA_WARP) {
+    const uint32_t id = dcu::idesc(BF16, COLS, false);
+    const uint64_t dq = dcu::desc(dcp::smem_u32(ring), 0);
+    bool ok = true;
+    auto scores = [&](int g, int i) {
+      const int st = i % C::STAGES;
+      // (lanes by turns: the tile is here, the group's scores before have been read)
+      const bool odd = lane & 1;
+      if (!__all_sync(~0u, dcp::mbar_wait(odd ? &s_free[g] : &full[st], odd ? i & 1 : (i / C::STAGES) & 1, a.status)))
+        return false;
+      dcu::fence_after();
+      if (dcu::elect()) {
+#pragma unroll
+        for (int kk = 0; kk < 4 * NP; kk++)
+          dcu::mma_ts(tmem + s_col(g), tmem + k_col(g) + kk * 8,
+                      dq + st * (C::TILE >> 4) + (((kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), id, kk > 0);
+        dcu::commit(&s_full[g]);
+        if (g == groups - 1) dcu::commit(&empty[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    // the second group a tile behind: its first scores wait until the first
+    // group has read its own, so one's exponentials fill the other's waits
+    for (int i = 0; i < n + groups - 1 && ok; i++) {
+      if (i < n) ok = scores(0, i);
+      if (ok && groups == 2 && i > 0) ok = scores(1, i - 1);
+    }
+  } else if (warp >= EXP_WARP && (warp - EXP_WARP) >> 2 < groups) {
+    const int g = (warp - EXP_WARP) >> 2, quarter = warp & 3, me = threadIdx.x - 32 * EXP_WARP - 128 * g;
+    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int key = k0 + g * KEYS + quarter * 32 + lane;
+    // ---- this thread's key into TMEM (once a block; zeros behind the cache's end)
+    {
+      const uint4* src = (const uint4*)((const uint16_t*)a.k + b * a.k_seq + (int64_t)key * a.k_tok + h * a.k_head);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        uint32_t r[32];
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (key < a.cache && (8 * p + x) * 8 < a.hd) v = src[8 * p + x];
+          r[4 * x] = v.x, r[4 * x + 1] = v.y, r[4 * x + 2] = v.z, r[4 * x + 3] = v.w;
+        }
+        dcu::st32(lane_at + k_col(g) + 32 * p, r);
+      }
+      dcu::wait_st();
+      dcu::fence_before();
+      __syncwarp();
+      if (lane == 0) dcp::mbar_arrive(&s_free[g]);
+    }
+    const int64_t lse_at = (int64_t)b * a.rows * a.heads + h * a.group;
+    float* L2 = scales + g * 2 * COLS;
+    float next = lse_of(a, lse_at, t0, me), sum = 0.0f;
+    bool ok = true;  // (a warp whose wait gave up stays in the loop: the others count on it at the barrier)
+    for (int i = 0; i < n; i++) {
+      float* L = L2 + (i & 1) * COLS;
+      L[me] = scale_of(next);
+      if (i + 1 < n) next = lse_of(a, lse_at, t0 + i + 1, me);  // (used a tile later)
+      // (one barrier a tile: who passes it has read the buffer of two tiles ago)
+      dcp::named_sync(1 + g, 128);
+      ok = ok && __all_sync(~0u, dcp::mbar_wait(&s_full[g], i & 1, a.status));
+      if (!ok) continue;
+      dcu::fence_after();
+      const int first_row = (t0 + i) * a.tile_rows;
+      const int from = a.causal ? max(0, key - len + a.rows - first_row) * a.group : 0;  // columns that see the key
+      const int cols = min(a.tile_cols, (a.rows - first_row) * a.group);
+      const bool late = __any_sync(~0u, from > 0);
+      F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
+#pragma unroll 1
+      for (int c0 = 0; c0 < COLS; c0 += 64) {
+        uint32_t x[32], y[32];
+        dcu::ld32(lane_at + s_col(g) + c0, x);
+        dcu::ld32(lane_at + s_col(g) + c0 + 32, y);
+        dcu::wait_ld(x);
+        dcu::wait_ld(y);
+        if (c0 == 64) {
+          // the next tile's products run under the rest of this one's exponentials
+          dcu::fence_before();
+          __syncwarp();
+          if (lane == 0) dcp::mbar_arrive(&s_free[g]);
+        }
+        if (c0 < cols) add_columns<MANY_EVERY>(part, x, L, a.c, c0, from, cols, late);
+        if (c0 + 32 < cols) add_columns<MANY_EVERY>(part, y, L, a.c, c0 + 32, from, cols, late);
+      }
+      sum += sum_of(part);
+    }
+    if (ok && key < len) put(a, b, h, key, sum);
+  }
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    dcu::fence_after();
+    dcu::dealloc(tmem, 512);
   }
 }
 
 template <int NP, bool BF16>
-int run(dc_ctx* ctx, const CUtensorMap& k, const CUtensorMap& q, const CwArgs& a, int64_t blocks, bool keep_q) {
+int run(dc_ctx* ctx, const CUtensorMap& k, const CUtensorMap& q, const CwArgs& a, int64_t blocks, bool few) {
   const dim3 grid((unsigned)blocks);
-  return keep_q ? launch(ctx, k_cache_weights<NP, BF16, true>, grid, THREADS, Cfg<NP, true>::SMEM, 1, k, q, a)
-                : launch(ctx, k_cache_weights<NP, BF16, false>, grid, THREADS, Cfg<NP, false>::SMEM, 1, k, q, a);
+  return few ? launch(ctx, k_weights_few<NP, BF16>, grid, FEW_THREADS, FEW_SMEM<NP>, 1, k, q, a)
+             : launch(ctx, k_weights_many<NP, BF16>, grid, MANY_THREADS, Many<NP>::SMEM, 1, q, a);
 }
 
 }  // namespace
@@ -305,22 +446,20 @@ extern "C" int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* p) {
   CwArgs a;
   a.group = A.heads / A.kv_heads;
   a.tile_rows = COLS / a.group;
-  const bool keep_q = A.rows <= a.tile_rows;
-  if (keep_q) a.tile_rows = A.rows;
+  const bool few = A.rows <= a.tile_rows;
+  if (few) a.tile_rows = A.rows;
   a.tile_cols = a.tile_rows * a.group;
   a.col_tiles = (A.rows + a.tile_rows - 1) / a.tile_rows;
   a.cols_mma = (a.tile_cols + 31) / 32 * 32;  // (columns are read 32 at a time)
   const int64_t heads = (int64_t)A.batch * A.kv_heads, tiles = (A.cache + KEYS - 1) / KEYS;
-  // keep_q: one wave of two blocks an SM, each an even share of a head's key
-  // tiles; else a block for every key tile
-  int64_t splits = tiles;
-  if (keep_q) {
+  // few: one wave of two blocks an SM, each an even share of a head's key
+  // tiles; many: a block for every two key tiles
+  int64_t splits = (tiles + 1) / 2;
+  if (few) {
     splits = std::min(tiles, std::max<int64_t>(1, 2 * (int64_t)ctx->sm_count / heads));
     const int64_t each = (tiles + splits - 1) / splits;
     splits = (tiles + each - 1) / each;
     a.chunk = (int)(each * KEYS);
-  } else {
-    a.chunk = KEYS;
   }
   a.splits = (int)splits;
   if (heads * splits > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "cache_weights: too many blocks");
@@ -337,13 +476,14 @@ extern "C" int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* p) {
   const uint32_t bq[5] = {64, (uint32_t)a.group, 1, (uint32_t)a.tile_rows, 1};
   if (!dcu::encode(&mk, A.k, bf16, 4, dk, sk, bk) || !dcu::encode(&mq, A.q, bf16, 5, dq, sq, bq))
     return dc_fail(ctx, DC_E_INVAL, "cache_weights: these q or k strides make no tensor map");
+  a.k = A.k, a.k_seq = A.k_seq, a.k_tok = A.k_tok, a.k_head = A.k_head, a.hd = A.head_dim;
   a.lens = A.lens, a.lse = A.lse, a.acc = A.acc, a.acc_seq = A.acc_seq, a.acc_head = A.acc_head;
   a.c = c, a.decay = (float)A.decay;
   a.rows = A.rows, a.heads = A.heads, a.kv_heads = A.kv_heads, a.cache = A.cache, a.causal = A.causal != 0;
   a.status = ctx->d_status;
   if (A.head_dim <= 64)
-    return bf16 ? run<1, true>(ctx, mk, mq, a, heads * splits, keep_q)
-                : run<1, false>(ctx, mk, mq, a, heads * splits, keep_q);
-  return bf16 ? run<2, true>(ctx, mk, mq, a, heads * splits, keep_q)
-              : run<2, false>(ctx, mk, mq, a, heads * splits, keep_q);
+    return bf16 ? run<1, true>(ctx, mk, mq, a, heads * splits, few)
+                : run<1, false>(ctx, mk, mq, a, heads * splits, few);
+  return bf16 ? run<2, true>(ctx, mk, mq, a, heads * splits, few)
+              : run<2, false>(ctx, mk, mq, a, heads * splits, few);
 }
