@@ -168,17 +168,23 @@ class Compute:
         t = Compute._type_of
         if not t:
             import torch
-            t.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, "i32": torch.int32, "i64": torch.int64})
+            t.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, "i32": torch.int32, "i64": torch.int64,
+                      "u8": torch.uint8, "torch": torch})
         return t
 
     _type_of: dict = {}
 
     def _ptrs(self, what: str, *tensors) -> list:
         """The tensors' addresses (0 for None), all on this object's device."""
+        dev, at = self.device, []
         for t in tensors:
-            if t is not None and t.get_device() != self.device:
-                raise ValueError(f"{what}: a tensor is not on cuda:{self.device}")
-        return [t.data_ptr() if t is not None else 0 for t in tensors]
+            if t is None:
+                at.append(0)
+            elif t.get_device() == dev:
+                at.append(t.data_ptr())
+            else:
+                raise ValueError(f"{what}: a tensor is not on cuda:{dev}")
+        return at
 
     @staticmethod
     def _flat(t, shape, dtype) -> bool:
@@ -186,13 +192,16 @@ class Compute:
 
     def _scratch(self, n: int):
         """n bytes of torch's memory, in the order of the stream that this object launches on."""
-        import torch
-        here = torch.cuda.current_stream(self.device)
-        stream = self.L.dc_stream(self.h)
-        if (here.cuda_stream or 1) == (stream or 1):
-            return torch.empty(n, dtype=torch.uint8, device=here.device)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
-            return torch.empty(n, dtype=torch.uint8, device=here.device)
+        T = self._types()
+        torch, stream = T["torch"], self.L.dc_stream(self.h)
+        dev = T.get(self.device)
+        if dev is None:
+            dev = T[self.device] = torch.device("cuda", self.device)
+        # (the legacy default stream is 0 to torch and 1 to the library)
+        if (torch._C._cuda_getCurrentRawStream(self.device) or 1) == (stream or 1):
+            return torch.empty(n, dtype=T["u8"], device=dev)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)):
+            return torch.empty(n, dtype=T["u8"], device=dev)
 
     def head_norm_rope_dev(self, x, pos, q, k, v, slots=None, *, wq=None, wk=None, eps=1e-5, theta=10000.0,
                            inv_freq=None, rot=None, sections=None, cyclic: bool = False) -> None:
@@ -270,11 +279,14 @@ class Compute:
         a = self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale)
         if ws is None:
             n = self.L.dc_prefix_attention_ws(self.h, a)
-            ws = self._scratch(n) if n else None
-        elif not ws.is_contiguous():
+            if n:
+                ws = self._scratch(n)
+        elif ws.is_contiguous():
+            self._ptrs("prefix_attention", ws)
+            n = ws.numel() * ws.element_size()
+        else:
             raise ValueError("prefix_attention: ws is contiguous")
-        at, = self._ptrs("prefix_attention", ws)
-        rc = self.L.dc_prefix_attention_dev(self.h, a, at, ws.numel() * ws.element_size() if at else 0)
+        rc = self.L.dc_prefix_attention_dev(self.h, a, ws.data_ptr() if n else None, n)
         if rc:
             self._check(rc, "prefix_attention")
 
