@@ -8,7 +8,8 @@
 //   * k_shared: the rows of all sequences that use one key/value head, 128 or 256
 //     a block, against a range of the prefix: one reading of its keys and values
 //     for the whole batch;
-//   * k_own: a sequence's rows that use one head against a range of its own keys;
+//   * k_own: a sequence's rows that use one head against a range of its own keys
+//     (and a batch's few rows against the prefix);
 //   * k_join: the parts of a row, and its last tokens (below).
 //
 // A running maximum is raised only when a row's has grown by more than 2^8:
@@ -54,8 +55,8 @@ struct PaArgs {
   float c;  // scale * log2 e
   int batch, rows, heads, kv_heads, group, hd, prefix, own_max;
   int pre_rows, pre_m, pre_chunk, pre_splits;  // rows a head, row tiles, keys a split, splits
-  int pre_halves;                              // parts of a split (2 where a row tile has a block of its own)
   int own_rows, own_m, own_chunk, own_splits;
+  int few_blocks;    // blocks of k_own that take the prefix
   int64_t own_base;  // first own part
   int* status;
 };
@@ -94,8 +95,7 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 //   S = Q K^T (128 x 128, f32 in TMEM),  O += P V (128 x hd in TMEM)
 // with P rounded to the keys' type.  With two tiles of rows each group has its
 // own and both use each tile of keys; a tile of rows that is left over has a block
-// whose groups take every other tile of keys, and its own part of the result
-// each.  One group's softmax runs under the other's products.
+// whose groups take every other tile of keys and join their parts.  One group's softmax runs under the other's products.
 //
 // One block an SM (224 KB, all 512 TMEM columns).  Heads up to 64 wide leave room
 // for P beside S: the next scores are formed as soon as these have been read.
@@ -396,28 +396,71 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
       l += both.x + both.y;
       if (!met) { ok = false; break; }
     }
-    if (used) {
-      const int row = quarter * 32 + lane;
-      const int half = two ? 0 : g;
-      const int64_t part = ((int64_t)(split * a.pre_halves + half) * a.kv_heads + h) * a.pre_rows + m * ROWS + row;
-      if (count > 0 && ok && warp_wait(&o_done[g], (count - 1) & 1, a.status)) {
-        dcu::fence_after();
-        float* dst = a.part_o + part * C::WIDTH;
+    // ---- the part: through shared memory (the ring, once both groups are done
+    // with it), a row to a thread, each then one bulk copy; two groups of one tile
+    // of rows join theirs first.  (Stored from registers, 16 bytes a row at a
+    // time, this took 2.9 us of a block's 15 at four tiles a block.)
+    constexpr int STRIDE = C::WIDTH * 4 + 16;  // rows of neighbouring lanes in different banks
+    static_assert(2 * 128 * STRIDE <= C::STAGES * C::TILE, "the ring holds both groups' parts");
+    const int row = quarter * 32 + lane;
+    uint8_t* mine = ring + (g * 128 + row) * STRIDE;
+    ok = ok && count > 0 && used && warp_wait(&o_done[g], (count - 1) & 1, a.status);
+    if (!ok) mx = -INFINITY, l = 0.0f;
+    float2 ml = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
+    dcp::named_sync(1, 256);
+    dcu::fence_after();
+    // this row, times f, and (join) the second group's, times f_other; a factor of
+    // 0 means a part without weight, whose O may be anything
+    auto put = [&](bool join, float f, float f_other) {
+      const uint8_t* other = mine + 128 * STRIDE;
 #pragma unroll 1
-        for (int col = 0; col < C::WIDTH; col += 32) {
-          uint32_t o[32];
-          dcu::ld32(o_at + col, o);
-          dcu::wait_ld(o);
-          if (row < nrows) {
+      for (int col = 0; col < C::WIDTH; col += 16) {
+        uint32_t o[16];
+        dcu::ld16(o_at + col, o);
+        dcu::wait_ld(o);
 #pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              *reinterpret_cast<uint4*>(dst + col + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+        for (int y = 0; y < 16; y += 4) {
+          float4 v = make_float4(0, 0, 0, 0);
+          if (f != 0.0f)
+            v = make_float4(f * __uint_as_float(o[y]), f * __uint_as_float(o[y + 1]), f * __uint_as_float(o[y + 2]),
+                            f * __uint_as_float(o[y + 3]));
+          if (join && f_other != 0.0f) {
+            const float4 w = *reinterpret_cast<const float4*>(other + (col + y) * 4);
+            v.x = fmaf(f_other, w.x, v.x), v.y = fmaf(f_other, w.y, v.y);
+            v.z = fmaf(f_other, w.z, v.z), v.w = fmaf(f_other, w.w, v.w);
           }
+          *reinterpret_cast<float4*>(mine + (col + y) * 4) = v;
         }
-      } else {
-        mx = -INFINITY, l = 0.0f;
       }
-      if (row < nrows) a.part_ml[part] = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
+    };
+    if (!two) {
+      if (g == 1) {
+        if (ok) put(false, 1.0f, 0.0f);
+        *reinterpret_cast<float2*>(mine + C::WIDTH * 4) = ml;
+      }
+      dcp::named_sync(1, 256);
+    }
+    if (two || g == 0) {
+      const int64_t part = ((int64_t)split * a.kv_heads + h) * a.pre_rows + m * ROWS + row;
+      if (ok) {
+        float f = 1.0f, f_other = 0.0f;
+        if (!two) {
+          const float2 x = *reinterpret_cast<const float2*>(mine + 128 * STRIDE + C::WIDTH * 4);
+          const float top = fmaxf(ml.x, x.x), base = top == -INFINITY ? 0.0f : top;
+          f = ml.y == 0.0f ? 0.0f : dcu::ex2(ml.x - base);
+          f_other = x.y == 0.0f ? 0.0f : dcu::ex2(x.x - base);
+          ml = make_float2(top, fmaf(f_other, x.y, f * ml.y));
+        }
+        put(!two, f, f_other);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (row < nrows)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + part * C::WIDTH),
+                       "r"(dcp::smem_u32(mine)), "r"(C::WIDTH * 4)
+                       : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      }
+      if (row < nrows) a.part_ml[part] = ml;
     }
     dcu::fence_before();
   }
@@ -437,6 +480,14 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
 // these, and its round trips through TMEM cost more than the copies: 41 us
 // against HBM's 21 for 64 sequences of up to 1024 tokens).  The warps' results
 // join in shared memory.
+//
+// Where the whole batch has up to FEW_ROWS rows a head, its prefix is taken here
+// too, as if it were one sequence's own keys: a tile of 128 rows would be mostly
+// empty, and its setup and first products cost more than reading the keys.  8
+// key heads of 128 columns, this way and k_shared's, us: 4 rows on 333 keys 5.9
+// and 9.6, on 8192 13.0 and 15.4, on 65536 49.9 and 49.1; 32 rows 6.9 and 10.6,
+// 15.4 and 17.9, 50.9 and 53.1; 64 rows 8.1 and 10.6, 19.3 and 18.3, 87 and 54.
+constexpr int FEW_ROWS = 32;
 constexpr int OWN_ROWS = 16;
 constexpr int OWN_KEYS = 16;
 constexpr int OWN_WARPS = 4;
@@ -482,7 +533,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // `behind`: launched behind k_shared, whose end it waits for last.
 template <int NP, bool BF16>
 __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
-    k_own(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+    k_own(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
+          const __grid_constant__ CUtensorMap map_ko, const __grid_constant__ CUtensorMap map_vo,
           const __grid_constant__ PaArgs a, const int behind) {
   using C = Own<NP>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -490,14 +542,30 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (!behind) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  int t = blockIdx.x;
-  const int m = t % a.own_m;
-  t /= a.own_m;
-  const int split = t % a.own_splits, bh = t / a.own_splits, h = bh % a.kv_heads, seq = bh / a.kv_heads;
-  const int seen = max(0, min(a.lens[seq], a.own_max) - (a.rows - 1));  // tokens that all rows see
-  const int k0 = split * a.own_chunk, k1 = min(seen, k0 + a.own_chunk);
-  const int nrows = min(OWN_ROWS, a.own_rows - m * OWN_ROWS);
-  const int64_t part = a.own_base + (int64_t)t * a.own_rows + m * OWN_ROWS;
+  const bool pre = (int)blockIdx.x < a.few_blocks;
+  const int row_tiles = pre ? a.pre_m : a.own_m, splits = pre ? a.pre_splits : a.own_splits;
+  int t = blockIdx.x - (pre ? 0 : a.few_blocks);
+  const int m = t % row_tiles;
+  t /= row_tiles;
+  int split, h, seq = -1, k0, k1, rows;
+  int64_t part;
+  if (pre) {
+    h = t % a.kv_heads, split = t / a.kv_heads;
+    k0 = split * a.pre_chunk, k1 = min(a.prefix, k0 + a.pre_chunk);
+    rows = a.pre_rows;
+    part = (int64_t)t * rows;
+  } else {
+    split = t % splits;
+    const int bh = t / splits;
+    h = bh % a.kv_heads, seq = bh / a.kv_heads;
+    const int seen = max(0, min(a.lens[seq], a.own_max) - (a.rows - 1));  // tokens that all rows see
+    k0 = split * a.own_chunk, k1 = min(seen, k0 + a.own_chunk);
+    rows = a.own_rows;
+    part = a.own_base + (int64_t)t * rows;
+  }
+  const int nrows = min(OWN_ROWS, rows - m * OWN_ROWS);
+  part += m * OWN_ROWS;
+  const CUtensorMap *map_k = pre ? &map_kp : &map_ko, *map_v = pre ? &map_vp : &map_vo;
   if (k1 <= k0) {
     if ((int)threadIdx.x < nrows) a.part_ml[part + threadIdx.x] = make_float2(-INFINITY, 0.0f);
   } else {
@@ -511,8 +579,8 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
 #pragma unroll
       for (int p = 0; p < NP; p++) {
         uint8_t* dst = ring + st * 2 * C::TILE + p * C::PANEL;
-        dcu::tma_load_4d(dst, &map_k, p * 64, h, key_of(i), seq, &full[st]);
-        dcu::tma_load_4d(dst + C::TILE, &map_v, p * 64, h, key_of(i), seq, &full[st]);
+        dcu::tma_load_4d(dst, map_k, p * 64, h, key_of(i), pre ? 0 : seq, &full[st]);
+        dcu::tma_load_4d(dst + C::TILE, map_v, p * 64, h, key_of(i), pre ? 0 : seq, &full[st]);
       }
     };
     if (lane == 0) {
@@ -679,16 +747,12 @@ __global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) 
   if (id >= (int64_t)a.batch * a.rows * a.heads) return;
   const int head = id % a.heads, br = id / a.heads, r = br % a.rows, b = br / a.rows;
   const int h = head / a.group, g = head - h * a.group;
-  // parts: of the prefix's splits (both halves where the row's tile has a block
-  // of its own), then of the own splits
-  const int row = br * a.group + g;
-  const int halves = a.pre_halves == 2 && row / ROWS == a.pre_m - 1 ? 2 : 1;
-  const int pre = a.pre_splits * halves, total = pre + a.own_splits;
+  // parts: of the prefix's splits, then of the own splits
+  const int total = a.pre_splits + a.own_splits;
+  const int64_t pre_at = (int64_t)h * a.pre_rows + br * a.group + g, pre_step = (int64_t)a.kv_heads * a.pre_rows;
   const int64_t own_at = a.own_base + (int64_t)(b * a.kv_heads + h) * a.own_splits * a.own_rows + r * a.group + g;
   auto at = [&](int i) {
-    if (i >= pre) return own_at + (int64_t)(i - pre) * a.own_rows;
-    const int64_t part = halves == 2 ? i : i * a.pre_halves;
-    return (part * a.kv_heads + h) * a.pre_rows + row;
+    return i < a.pre_splits ? pre_at + i * pre_step : own_at + (int64_t)(i - a.pre_splits) * a.own_rows;
   };
   // the tail's scores, lane j that of token j
   int tail0 = 0, tail = 0;
@@ -780,9 +844,10 @@ __global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) 
 // How a call's keys are split: the splits follow from sizes alone, so that the
 // workspace's size is known before the call.
 struct Plan {
-  int group, pre_rows, pre_m, pre_chunk, pre_splits, pre_halves, own_rows, own_m, own_chunk, own_splits;
+  int group, pre_rows, pre_m, pre_chunk, pre_splits, own_rows, own_m, own_chunk, own_splits;
   int64_t pre_blocks, own_blocks, own_base, parts;
   int width;
+  bool few;  // the prefix goes to k_own
 };
 // The number of even shares of `tiles` tiles for each of `items`, `slots` blocks
 // at a time, that ends first: a block costs `start` tiles beside its own (TMEM,
@@ -808,17 +873,18 @@ Plan make_plan(const dc_prefix_attn& A, int sm_count) {
     return (int)((tiles + each - 1) / each);
   };
   p.pre_rows = A.batch * A.rows * p.group;
-  p.pre_m = (p.pre_rows + ROWS - 1) / ROWS;
-  p.pre_halves = 1 + (p.pre_m & 1);
-  const int64_t tp = (A.prefix + KEYS - 1) / KEYS, hp = (int64_t)A.kv_heads * ((p.pre_m + 1) / 2);
-  p.pre_splits = split(tp, shares(hp, tp, sm_count, 3), KEYS, &p.pre_chunk);
+  p.few = p.pre_rows <= FEW_ROWS;
+  const int tile = p.few ? OWN_STEP : KEYS;
+  p.pre_m = (p.pre_rows + (p.few ? OWN_ROWS : ROWS) - 1) / (p.few ? OWN_ROWS : ROWS);
+  const int64_t tp = (A.prefix + tile - 1) / tile, hp = (int64_t)A.kv_heads * (p.few ? p.pre_m : (p.pre_m + 1) / 2);
+  p.pre_splits = split(tp, p.few ? shares(hp, tp, 2 * sm_count, 4) : shares(hp, tp, sm_count, 3), tile, &p.pre_chunk);
   p.own_rows = A.rows * p.group;
   p.own_m = (p.own_rows + OWN_ROWS - 1) / OWN_ROWS;
   const int64_t to = (A.own_max + OWN_STEP - 1) / OWN_STEP, ho = (int64_t)A.batch * A.kv_heads * p.own_m;
   p.own_splits = split(to, shares(ho, to, 2 * sm_count, 4), OWN_STEP, &p.own_chunk);
   p.pre_blocks = hp * p.pre_splits;
   p.own_blocks = ho * p.own_splits;
-  p.own_base = (int64_t)p.pre_splits * p.pre_halves * A.kv_heads * p.pre_rows;
+  p.own_base = (int64_t)p.pre_splits * A.kv_heads * p.pre_rows;
   p.parts = p.own_base + (int64_t)A.batch * A.kv_heads * p.own_splits * p.own_rows;
   return p;
 }
@@ -845,13 +911,15 @@ size_t ws_bytes_of(const Plan& p) { return (size_t)p.parts * (p.width * 4 + 8); 
 template <int NP, bool BF16>
 int run(dc_ctx* ctx, const CUtensorMap (&maps)[4], const PaArgs& a, const Plan& p, bool f32_out) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  if (p.pre_blocks)
+  const bool shared = p.pre_blocks && !p.few;
+  const int64_t own = p.own_blocks + (p.few ? p.pre_blocks : 0);
+  if (shared)
     if (int rc = launch(ctx, k_shared<NP, BF16>, dim3((unsigned)p.pre_blocks), SH_THREADS, Shared<NP>::SMEM, 1, maps[0],
                         maps[1], a))
       return rc;
-  if (p.own_blocks)
-    if (int rc = launch(ctx, k_own<NP, BF16>, dim3((unsigned)p.own_blocks), OWN_WARPS * 32, Own<NP>::SMEM, 1, maps[2],
-                        maps[3], a, (int)(p.pre_blocks > 0)))
+  if (own)
+    if (int rc = launch(ctx, k_own<NP, BF16>, dim3((unsigned)own), OWN_WARPS * 32, Own<NP>::SMEM, 1, maps[0], maps[1],
+                        maps[2], maps[3], a, (int)shared))
       return rc;
   const dim3 grid((unsigned)(((int64_t)a.batch * a.rows * a.heads + 3) / 4));
   return f32_out ? launch(ctx, k_join<NP, T, float>, grid, 128, 0, 1, a)
@@ -915,13 +983,15 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
   CUtensorMap maps[4];
   memset(maps, 0, sizeof maps);
   const uint64_t hd = A.head_dim, kv = A.kv_heads;
-  const uint32_t box[3] = {64, 1, KEYS}, own_box[4] = {64, 1, OWN_KEYS, 1};
+  const uint32_t own_box[4] = {64, 1, OWN_KEYS, 1}, box[3] = {64, 1, KEYS};
   bool ok = true;
   if (A.prefix) {
-    const uint64_t dims[3] = {hd, kv, (uint64_t)A.prefix};
-    const uint64_t sk[2] = {2 * (uint64_t)A.kp_head, 2 * (uint64_t)A.kp_tok};
-    const uint64_t sv[2] = {2 * (uint64_t)A.vp_head, 2 * (uint64_t)A.vp_tok};
-    ok = dcu::encode(&maps[0], A.k_pre, bf16, 3, dims, sk, box) && dcu::encode(&maps[1], A.v_pre, bf16, 3, dims, sv, box);
+    const uint64_t dims[4] = {hd, kv, (uint64_t)A.prefix, 1};
+    const uint64_t sk[3] = {2 * (uint64_t)A.kp_head, 2 * (uint64_t)A.kp_tok, 0};
+    const uint64_t sv[3] = {2 * (uint64_t)A.vp_head, 2 * (uint64_t)A.vp_tok, 0};
+    const int rank = pl.few ? 4 : 3;  // (k_own takes a sequence's number too)
+    ok = dcu::encode(&maps[0], A.k_pre, bf16, rank, dims, sk, pl.few ? own_box : box) &&
+         dcu::encode(&maps[1], A.v_pre, bf16, rank, dims, sv, pl.few ? own_box : box);
   }
   if (A.own_max) {
     const uint64_t dims[4] = {hd, kv, (uint64_t)A.own_max, (uint64_t)A.batch};
@@ -944,10 +1014,10 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
   a.batch = A.batch, a.rows = A.rows, a.heads = A.heads, a.kv_heads = A.kv_heads, a.group = pl.group;
   a.hd = A.head_dim, a.prefix = A.prefix, a.own_max = A.own_max;
   a.pre_rows = pl.pre_rows, a.pre_m = pl.pre_m, a.pre_chunk = pl.pre_chunk, a.pre_splits = pl.pre_splits;
-  a.pre_halves = pl.pre_halves;
   a.own_rows = pl.own_rows, a.own_m = pl.own_m, a.own_chunk = pl.own_chunk, a.own_splits = pl.own_splits;
   a.own_base = pl.own_base, a.status = ctx->d_status;
-  if (std::max(pl.pre_blocks, pl.own_blocks) > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: too many blocks");
+  a.few_blocks = pl.few ? (int)pl.pre_blocks : 0;
+  if (pl.pre_blocks + pl.own_blocks > INT32_MAX) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: too many blocks");
   const bool f32_out = A.out_type == DC_F32;
   if (pl.width == 64)
     return bf16 ? run<1, true>(ctx, maps, a, pl, f32_out) : run<1, false>(ctx, maps, a, pl, f32_out);
