@@ -747,11 +747,29 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
 // One warp per (sequence, row, query head): joins the parts of its row, eight
 // in flight, and scores the own tokens behind those that all rows see.  A lane
 // holds WIDTH / 32 channels.
+//
+// Latency bounds it (a few hundred KB to 12 MB out of L2), so what does not hang
+// together is read at once: the last tokens before the parts are complete
+// (`behind`: an own kernel before this one has seen to it that q, the caches and
+// lens are), the first parts beside their maxima and sums.
+template <typename T, int E>
+__device__ __forceinline__ void load_f32(const T* src, float (&v)[E]) {  // aligned to its E values
+  uint32_t raw[E / 2];
+  if constexpr (E == 4) {
+    const uint2 x = *reinterpret_cast<const uint2*>(src);
+    raw[0] = x.x, raw[1] = x.y;
+  } else {
+    raw[0] = *reinterpret_cast<const uint32_t*>(src);
+  }
+  const T* t = reinterpret_cast<const T*>(raw);
+#pragma unroll
+  for (int e = 0; e < E; e++) v[e] = to_f32(t[e]);
+}
 template <int NP, typename T, typename TO>
-__global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) {
-  constexpr int W = 64 * NP, E = W / 32;
+__global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a, const int behind) {
+  constexpr int W = 64 * NP, E = W / 32, EARLY = 4;
   asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!behind) asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (id >= (int64_t)a.batch * a.rows * a.heads) return;
@@ -766,28 +784,48 @@ __global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) 
   };
   // the tail's scores, lane j that of token j
   int tail0 = 0, tail = 0;
-  float sc = -INFINITY;
+  float sc = -INFINITY, late[EARLY][E];  // (values of the first few)
   const int c0 = lane * E;
+  const bool in = c0 < a.hd;  // (all of a lane's channels, or none: hd is a multiple of 8)
+  const T* vp = (const T*)a.v_own + b * a.vo_seq + h * a.vo_head;
   if (a.own_max > 0 && r > 0) {
     const int len = max(0, min(a.lens[b], a.own_max));
     tail0 = max(0, len - (a.rows - 1));
     tail = max(0, len - (a.rows - 1 - r) - tail0);
-    float q[E];
-    const T* qp = (const T*)a.q + b * a.q_seq + r * a.q_row + (int64_t)head * a.q_head;
-#pragma unroll
-    for (int e = 0; e < E; e++) q[e] = c0 + e < a.hd ? to_f32(qp[c0 + e]) : 0.0f;
+    float q[E] = {};
+    if (in) load_f32((const T*)a.q + b * a.q_seq + r * a.q_row + (int64_t)head * a.q_head + c0, q);
     const T* kp = (const T*)a.k_own + b * a.ko_seq + h * a.ko_head;
+#pragma unroll
+    for (int j = 0; j < EARLY; j++)
+      if (in && j < tail) load_f32(vp + (tail0 + j) * a.vo_tok + c0, late[j]);
 #pragma unroll 4
     for (int j = 0; j < tail; j++) {
-      float s = 0.0f;
+      float s = 0.0f, k[E];
+      if (in) {
+        load_f32(kp + (tail0 + j) * a.ko_tok + c0, k);
 #pragma unroll
-      for (int e = 0; e < E; e++)
-        if (c0 + e < a.hd) s = fmaf(q[e], to_f32(kp[(tail0 + j) * a.ko_tok + c0 + e]), s);
+        for (int e = 0; e < E; e++) s = fmaf(q[e], k[e], s);
+      }
 #pragma unroll
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
       if (lane == j) sc = s * a.c;
     }
   }
+  if (behind) asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto part = [&](int i, float (&v)[E]) {
+    const float* o = a.part_o + at(i) * W + c0;
+    if constexpr (E == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(o);
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+      const float2 f = *reinterpret_cast<const float2*>(o);
+      v[0] = f.x, v[1] = f.y;
+    }
+  };
+  float first[8][E];  // (those without weight are whatever was there, and left out below)
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    if (j < total) part(j, first[j]);
   float M = sc;
   for (int i = lane; i < total; i += 32) M = fmaxf(M, a.part_ml[at(i)].x);
 #pragma unroll
@@ -805,40 +843,41 @@ __global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a) 
     const unsigned some = __ballot_sync(~0u, ml.y != 0.0f);
     const int cnt = min(32, total - i0);
     for (int i = 0; i < cnt; i += 8) {
-      float v[8][E];
+      if (i0 + i > 0) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-#pragma unroll
-        for (int e = 0; e < E; e++) v[j][e] = 0.0f;
-        if (some >> (i + j) & 1) {
-          const float* o = a.part_o + at(i0 + i + j) * W + c0;
-          if constexpr (E == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(o);
-            v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
-          } else {
-            const float2 f = *reinterpret_cast<const float2*>(o);
-            v[j][0] = f.x, v[j][1] = f.y;
-          }
-        }
+        for (int j = 0; j < 8; j++)
+          if (some >> (i + j) & 1) part(i0 + i + j, first[j]);
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float wj = __shfl_sync(~0u, w, i + j);
+        if (some >> (i + j) & 1) {
 #pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = fmaf(wj, v[j][e], acc[e]);
+          for (int e = 0; e < E; e++) acc[e] = fmaf(wj, first[j][e], acc[e]);
+        }
       }
     }
   }
   if (tail > 0) {
     const float w = lane < tail ? dcu::ex2(sc - base) : 0.0f;
     L += w;
-    const T* vp = (const T*)a.v_own + b * a.vo_seq + h * a.vo_head;
-#pragma unroll 4
-    for (int j = 0; j < tail; j++) {
-      const float wj = __shfl_sync(~0u, w, j);
 #pragma unroll
-      for (int e = 0; e < E; e++)
-        if (c0 + e < a.hd) acc[e] = fmaf(wj, to_f32(vp[(tail0 + j) * a.vo_tok + c0 + e]), acc[e]);
+    for (int j = 0; j < EARLY; j++) {
+      const float wj = __shfl_sync(~0u, w, j);
+      if (in && j < tail) {
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = fmaf(wj, late[j][e], acc[e]);
+      }
+    }
+#pragma unroll 4
+    for (int j = EARLY; j < tail; j++) {
+      const float wj = __shfl_sync(~0u, w, j);
+      float v[E];
+      if (in) {
+        load_f32(vp + (tail0 + j) * a.vo_tok + c0, v);
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = fmaf(wj, v[e], acc[e]);
+      }
     }
   }
 #pragma unroll
@@ -932,8 +971,8 @@ int run(dc_ctx* ctx, const CUtensorMap (&maps)[4], const PaArgs& a, const Plan& 
                         maps[2], maps[3], a, (int)shared))
       return rc;
   const dim3 grid((unsigned)(((int64_t)a.batch * a.rows * a.heads + 3) / 4));
-  return f32_out ? launch(ctx, k_join<NP, T, float>, grid, 128, 0, 1, a)
-                 : launch(ctx, k_join<NP, T, T>, grid, 128, 0, 1, a);
+  return f32_out ? launch(ctx, k_join<NP, T, float>, grid, 128, 0, 1, a, (int)(shared || own))
+                 : launch(ctx, k_join<NP, T, T>, grid, 128, 0, 1, a, (int)(shared || own));
 }
 
 }  // namespace
