@@ -78,23 +78,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return r;
 }
 
-// A wait of a whole warp: true where every lane's wait was met.  A plain test goes
-// first: where the barrier is met it takes 41 cycles, the suspending one 89.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
-  uint32_t met;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(met)
-      : "r"(dcp::smem_u32(bar)), "r"(parity)
-      : "memory");
-  return __all_sync(~0u, met) || __all_sync(~0u, dcp::mbar_wait(bar, parity, status));
-}
-// The same for two barriers at once.
+// A wait of a whole warp for two barriers at once.
 __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py, int* status) {
   const bool odd = threadIdx.x & 1;
-  return warp_wait(odd ? y : x, odd ? py : px, status);
+  return dcu::warp_wait(odd ? y : x, odd ? py : px, status);
 }
 
 // ---- the shared prefix ----------------------------------------------------------
@@ -260,7 +247,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
         const uint64_t v = dv + st * (C::TILE >> 4);
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-          ok = ok && (half ? warp_wait(&p_ready[2 * g + 1], j & 1, a.status)
+          ok = ok && (half ? dcu::warp_wait(&p_ready[2 * g + 1], j & 1, a.status)
                            : warp_wait2(&p_ready[2 * g], j & 1, &full[st], (s / C::STAGES) & 1, a.status));
           if (!ok) break;
           dcu::fence_after();
@@ -310,7 +297,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     float mx = -INFINITY, l = 0.0f;  // the maximum in use (scores before c), the sum
     bool ok = true;
     for (int j = 0; j < count; j++) {
-      if (!warp_wait(&s_full[g], j & 1, a.status)) { ok = false; break; }
+      if (!dcu::warp_wait(&s_full[g], j & 1, a.status)) { ok = false; break; }
       dcu::fence_after();
       uint32_t s[4][32];
       if (used) {
@@ -347,7 +334,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
         } else if (__any_sync(~0u, top > mx && !((top - mx) * a.c <= RAISE))) {
           // O *= 2^(c (old - new)), once it holds the product of the tile before
           // (the next product needs these probabilities)
-          if (C::APART && !warp_wait(&o_done[g], (j - 1) & 1, a.status)) { ok = false; break; }
+          if (C::APART && !dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status)) { ok = false; break; }
           dcu::fence_after();
           const float up = fmaxf(mx, top);
           const float f = mx == -INFINITY ? 0.0f : mx == up ? 1.0f : dcu::ex2((mx - up) * a.c);
@@ -371,7 +358,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         // (a warp without rows waits too: its arrival belongs to this tile's phase)
-        if (C::APART && !used && half == 0 && j > 0) met = warp_wait(&o_done[g], (j - 1) & 1, a.status);
+        if (C::APART && !used && half == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
         if (used) {
 #pragma unroll
           for (int x = 2 * half; x < 2 * half + 2; x++) {
@@ -392,7 +379,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
               p[y] = pack2<BF16>(v.x, v.y);
             }
             // (beside the scores: where the product of the tile before has read the ones there)
-            if (C::APART && x == 0 && j > 0) met = warp_wait(&o_done[g], (j - 1) & 1, a.status);
+            if (C::APART && x == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
             dcu::fence_after();
             dcu::st16(p_at + x * 16, p);
           }
@@ -414,7 +401,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     static_assert(2 * 128 * STRIDE <= C::STAGES * C::TILE, "the ring holds both groups' parts");
     const int row = quarter * 32 + lane;
     uint8_t* mine = ring + (g * 128 + row) * STRIDE;
-    ok = ok && count > 0 && used && warp_wait(&o_done[g], (count - 1) & 1, a.status);
+    ok = ok && count > 0 && used && dcu::warp_wait(&o_done[g], (count - 1) & 1, a.status);
     if (!ok) mx = -INFINITY, l = 0.0f;
     float2 ml = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
     dcp::named_sync(1, 256);
@@ -622,7 +609,7 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
     const int key_k = (lane / 16) * 8 + lane % 8, key_v = ((lane / 8) & 1) * 8 + lane % 8;
     for (int i = 0; i < n; i++) {
       const int st = i % OWN_STAGES;
-      ok = warp_wait(&full[st], (i / OWN_STAGES) & 1, a.status);
+      ok = dcu::warp_wait(&full[st], (i / OWN_STAGES) & 1, a.status);
       if (!ok) break;
       const int nv = min(OWN_KEYS, k1 - key_of(i));
       const uint32_t k_at = dcp::smem_u32(ring + st * 2 * C::TILE), v_at = k_at + C::TILE;
@@ -885,8 +872,15 @@ __global__ void __launch_bounds__(128) k_join(const __grid_constant__ PaArgs a, 
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   TO* out = (TO*)a.out + b * a.out_seq + r * a.out_row + (int64_t)head * a.out_head;
 #pragma unroll
-  for (int e = 0; e < E; e++)
-    if (c0 + e < a.hd) out[c0 + e] = from_f32<TO>(L == 0.0f ? 0.0f : acc[e] * inv);
+  for (int e = 0; e < E; e++) acc[e] = L == 0.0f ? 0.0f : acc[e] * inv;
+  if (in) {
+    struct alignas(E * sizeof(TO)) Row {
+      TO v[E];
+    } row;
+#pragma unroll
+    for (int e = 0; e < E; e++) row.v[e] = from_f32<TO>(acc[e]);
+    *reinterpret_cast<Row*>(out + c0) = row;
+  }
   if (a.lse && lane == 0) a.lse[id] = L == 0.0f ? -INFINITY : (base + log2f(L)) * LN2;
 }
 

@@ -186,13 +186,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   } else if (warp == 5) {
     const uint32_t id = dcu::idesc(BF16, 0, false) | ((uint32_t)(a.cols_mma >> 3) << 17);
     const uint64_t dq = dcu::desc(dcp::smem_u32(kept), 0), dk = dcu::desc(dcp::smem_u32(ring), 0);
-    bool ok = __all_sync(~0u, dcp::mbar_wait(kept_full, 0, a.status));
+    bool ok = dcu::warp_wait(kept_full, 0, a.status);
     for (int i = 0; i < n && ok; i++) {
-      if (i >= 2) ok = __all_sync(~0u, dcp::mbar_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status));
+      if (i >= 2) ok = dcu::warp_wait(&s_free[i & 1], ((i >> 1) & 1) ^ 1, a.status);
 #pragma unroll
       for (int p = 0; p < NP; p++) {
         const int s = i * NP + p, st = s % STAGES;
-        ok = ok && __all_sync(~0u, dcp::mbar_wait(&full[st], (s / STAGES) & 1, a.status));
+        ok = ok && dcu::warp_wait(&full[st], (s / STAGES) & 1, a.status);
         if (!ok) break;
         dcu::fence_after();
         if (dcu::elect()) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
     const uint32_t lane_at = tmem + ((uint32_t)(warp * 32) << 16);
     const int cols = a.tile_cols;
     for (int i = 0; i < n; i++) {
-      if (!__all_sync(~0u, dcp::mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.status))) break;
+      if (!dcu::warp_wait(&s_full[i & 1], (i >> 1) & 1, a.status)) break;
       dcu::fence_after();
       const int key = k0 + i * KEYS + warp * 32 + lane;
       const int from = a.causal ? max(0, key - len + a.rows) * a.group : 0;  // columns that see the key
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
       const int st = i % C::STAGES;
       // (lanes by turns: the tile is here, the group's scores before have been read)
       const bool odd = lane & 1;
-      if (!__all_sync(~0u, dcp::mbar_wait(odd ? &s_free[g] : &full[st], odd ? i & 1 : (i / C::STAGES) & 1, a.status)))
+      if (!dcu::warp_wait(odd ? &s_free[g] : &full[st], odd ? i & 1 : (i / C::STAGES) & 1, a.status))
         return false;
       dcu::fence_after();
       if (dcu::elect()) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
       if (i + 1 < n) next = lse_of(a, lse_at, t0 + i + 1, me);  // (used a tile later)
       // (one barrier a tile: who passes it has read the buffer of two tiles ago)
       dcp::named_sync(1 + g, 128);
-      ok = ok && __all_sync(~0u, dcp::mbar_wait(&s_full[g], i & 1, a.status));
+      ok = ok && dcu::warp_wait(&s_full[g], i & 1, a.status);
       if (!ok) continue;
       dcu::fence_after();
       const int first_row = (t0 + i) * a.tile_rows;
