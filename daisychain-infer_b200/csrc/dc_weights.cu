@@ -5,19 +5,23 @@
 // With lse known the sum needs no running maximum and no second pass.  The
 // product is formed as K Q^T: keys on the 128 TMEM lanes, up to 128 query rows
 // (row, head of the group; heads innermost) on the columns.  A thread then holds
-// one key against all rows and adds its exponentials in a register: no
-// exchange, no atomics, one order of summation.
+// one key against all rows (many: two threads, half of the columns each, joined at
+// the end) and adds its exponentials in a register: no atomics, one order of
+// summation.
 //
 // k_weights_few, up to 128 columns: a block keeps Q in shared memory and streams
 // its share of the cache's keys (16 KB panels through a ring by TMA), two blocks an
 // SM, scores double-buffered in TMEM.  HBM-bound: each key is read once.
 //
-// k_weights_many: a block keeps 256 keys in TMEM, as the first operand, for two
-// groups of four warps, and streams Q tiles (out of L2) past both.  Bound by the
-// exponential unit, 16 a cycle and SM: 128 x 128 of them take 1024 cycles, their
-// products 500 and their operands 256 of shared memory's (with the keys in shared
-// memory too, in two blocks an SM, the operands and copies took 768 and the whole
-// 1980 a tile).
+// k_weights_many: a block keeps 128 keys in TMEM, as the first operand, and streams
+// Q tiles (out of L2) past them, half a tile's scores (64 columns) in each of three
+// buffers, so that the products run ahead of the exponentials.  Two blocks of eight
+// exponential warps an SM: the unit takes 16 a cycle and SM, 448 cycles a half tile
+// with one pair in eight on the multiply-add pipe, but a warp's loads, waits and
+// sums around 32 exponentials a thread take as long, and only other warps fill
+// them.  1024 rows of 32 heads over 16384 keys of 8: 185 us, 0.72 PFLOP/s (the
+// unit alone 117); with 64 columns a warp and half as many warps 214, with 256 keys
+// a block and two groups of four warps 228.
 //
 // One warp copies, one issues the products.  Every wait is bounded; a block whose
 // wait gives up ends, and dc_sync reports it.
@@ -34,7 +38,7 @@ using dcu::F2;
 constexpr int KEYS = 128;   // keys of a tile: the MMA's M
 constexpr int COLS = 128;   // query rows of a tile: its N
 constexpr int FEW_THREADS = 192;
-constexpr int MANY_EVERY = 4;
+constexpr int MANY_EVERY = 8;
 constexpr int PANEL_BYTES = 128 * 128;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -236,39 +240,45 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   }
 }
 
-// Blocks of 2 x 128 keys against all Q tiles.  TMEM columns of group g: its keys
-// (64 x 32 bits a lane), its scores.
-constexpr int MANY_THREADS = 384, MMA_WARP = 0, TMA_WARP = 1, EXP_WARP = 4;
-constexpr uint32_t k_col(int g) { return g * 64; }
-constexpr uint32_t s_col(int g) { return 128 + g * COLS; }
+// Blocks of 128 keys against all Q tiles, two an SM, a half tile (64 columns) at a
+// time.  TMEM columns: the keys (64 x 32 bits a lane), three half tiles' scores.
+// (One pair in eight by multiply-adds: 185 us as above; in six 186, in twelve 192,
+// in four 200, none 196.)
+constexpr int HALF = COLS / 2, BUFS = 3, SCALES = 4;
+constexpr int MANY_THREADS = 352, MMA_WARP = 0, TMA_WARP = 1, SCALE_WARP = 2, EXP_WARP = 3;
+constexpr uint32_t s_col(int i) { return 64 + i * HALF; }
 template <int NP>
 struct Many {
   static constexpr int TILE = NP * PANEL_BYTES;
-  static constexpr int STAGES = NP == 2 ? 6 : 8;
-  static constexpr int SMEM = STAGES * TILE + 2 * 2 * COLS * 4 + 256;
+  static constexpr int STAGES = NP == 2 ? 3 : 6;
+  static constexpr int BARS = 2 * STAGES + 2 * BUFS + 2 * SCALES + 1;
+  static constexpr int SMEM = STAGES * TILE + SCALES * COLS * 4 + KEYS * 4 + BARS * 8 + 8;
 };
 
 template <int NP, bool BF16>
-__global__ void __launch_bounds__(MANY_THREADS, 1)
+__global__ void __launch_bounds__(MANY_THREADS, 2)
     k_weights_many(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CwArgs a) {
   using C = Many<NP>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;
-  float* scales = (float*)(ring + C::STAGES * C::TILE);  // [2 groups][2 tiles][COLS]
-  uint64_t* full = (uint64_t*)(scales + 4 * COLS);
+  float* scales = (float*)(ring + C::STAGES * C::TILE);  // [SCALES tiles][COLS]
+  float* halves = scales + SCALES * COLS;                // [KEYS] sums of the second warps
+  uint64_t* full = (uint64_t*)(halves + KEYS);
   uint64_t* empty = full + C::STAGES;
-  uint64_t* s_full = empty + C::STAGES;  // [2] a group's scores are in TMEM
-  uint64_t* s_free = s_full + 2;         // [2] and have been read (first: its keys are there)
-  uint32_t* slot = (uint32_t*)(s_free + 2);
+  uint64_t* s_full = empty + C::STAGES;  // [BUFS] a half tile's scores are in TMEM
+  uint64_t* s_free = s_full + BUFS;      // [BUFS] and have been read
+  uint64_t* l_full = s_free + BUFS;      // [SCALES] a tile's scales are there
+  uint64_t* l_free = l_full + SCALES;    // [SCALES] and have been read
+  uint64_t* k_ready = l_free + SCALES;   // the keys are in TMEM
+  uint32_t* slot = (uint32_t*)(full + C::BARS);
 
   const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int split = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
   const int h = bg % a.kv_heads, b = bg / a.kv_heads;
   const int len = max(0, min(a.lens[b], a.cache));
-  const int k0 = split * 2 * KEYS;
+  const int k0 = split * KEYS;
   if (len <= k0) return;
-  const int groups = len > k0 + KEYS ? 2 : 1;
   // Q tiles from the first that holds a row which sees the block's first key
   const int t0 = a.causal ? max(0, k0 - len + a.rows) / a.tile_rows : 0, n = a.col_tiles - t0;
 
@@ -277,13 +287,18 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
       dcp::mbar_init(&full[i], 1);
       dcp::mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < BUFS; i++) {
       dcp::mbar_init(&s_full[i], 1);
-      dcp::mbar_init(&s_free[i], 4);
+      dcp::mbar_init(&s_free[i], 8);
     }
+    for (int i = 0; i < SCALES; i++) {
+      dcp::mbar_init(&l_full[i], 1);
+      dcp::mbar_init(&l_free[i], 8);
+    }
+    dcp::mbar_init(k_ready, 8);
     dcp::mbar_fence_init();
   }
-  if (warp == MMA_WARP) dcu::alloc(slot, 512);
+  if (warp == MMA_WARP) dcu::alloc(slot, 256);
   zero_rows(ring, C::STAGES * NP, a.tile_cols, MANY_THREADS);
   dcu::fence_before();
   __syncthreads();
@@ -309,42 +324,53 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
           dcp::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, a.status);
     }
   } else if (warp == MMA_WARP) {
-    const uint32_t id = dcu::idesc(BF16, COLS, false);
+    const uint32_t id = dcu::idesc(BF16, HALF, false);
     const uint64_t dq = dcu::desc(dcp::smem_u32(ring), 0);
-    bool ok = true;
-    auto scores = [&](int g, int i) {
-      const int st = i % C::STAGES;
-      // (lanes by turns: the tile is here, the group's scores before have been read)
-      const bool odd = lane & 1;
-      if (!dcu::warp_wait(odd ? &s_free[g] : &full[st], odd ? i & 1 : (i / C::STAGES) & 1, a.status))
-        return false;
+    bool ok = dcu::warp_wait(k_ready, 0, a.status);
+    for (int u = 0; u < 2 * n && ok; u++) {
+      const int i = u >> 1, st = i % C::STAGES, buf = u % BUFS;
+      // (lanes by turns: the tile is here, the scores before have been read)
+      const bool odd = (lane & 1) && u >= BUFS;
+      ok = dcu::warp_wait(odd ? &s_free[buf] : &full[st], odd ? (u / BUFS - 1) & 1 : (i / C::STAGES) & 1, a.status);
+      if (!ok) break;
       dcu::fence_after();
       if (dcu::elect()) {
 #pragma unroll
         for (int kk = 0; kk < 4 * NP; kk++)
-          dcu::mma_ts(tmem + s_col(g), tmem + k_col(g) + kk * 8,
-                      dq + st * (C::TILE >> 4) + (((kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), id, kk > 0);
-        dcu::commit(&s_full[g]);
-        if (g == groups - 1) dcu::commit(&empty[st]);
+          dcu::mma_ts(tmem + s_col(buf), tmem + kk * 8,
+                      dq + ((st * C::TILE + (u & 1) * HALF * 128 + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), id, kk > 0);
+        dcu::commit(&s_full[buf]);
+        if (u & 1) dcu::commit(&empty[st]);
       }
       __syncwarp();
-      return true;
-    };
-    // the second group a tile behind: its first scores wait until the first
-    // group has read its own, so one's exponentials fill the other's waits
-    for (int i = 0; i < n + groups - 1 && ok; i++) {
-      if (i < n) ok = scores(0, i);
-      if (ok && groups == 2 && i > 0) ok = scores(1, i - 1);
     }
-  } else if (warp >= EXP_WARP && (warp - EXP_WARP) >> 2 < groups) {
-    const int g = (warp - EXP_WARP) >> 2, quarter = warp & 3, me = threadIdx.x - 32 * EXP_WARP - 128 * g;
+  } else if (warp == SCALE_WARP) {
+    // ---- each Q tile's scales, a tile's lse read while the one before is waited for
+    const int64_t lse_at = (int64_t)b * a.rows * a.heads + h * a.group;
+    float next[COLS / 32];
+#pragma unroll
+    for (int x = 0; x < COLS / 32; x++) next[x] = lse_of(a, lse_at, t0, x * 32 + lane);
+    for (int i = 0; i < n; i++) {
+      const int st = i % SCALES;
+      if (i >= SCALES && !dcu::warp_wait(&l_free[st], ((i / SCALES) & 1) ^ 1, a.status)) break;
+#pragma unroll
+      for (int x = 0; x < COLS / 32; x++) {
+        scales[st * COLS + x * 32 + lane] = scale_of(next[x]);
+        if (i + 1 < n) next[x] = lse_of(a, lse_at, t0 + i + 1, x * 32 + lane);
+      }
+      __syncwarp();
+      if (lane == 0) dcp::mbar_arrive(&l_full[st]);
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - EXP_WARP) >> 2;  // TMEM lanes, half of a buffer's columns
     const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
-    const int key = k0 + g * KEYS + quarter * 32 + lane;
+    const int key = k0 + quarter * 32 + lane;
     // ---- this thread's key into TMEM (once a block; zeros behind the cache's end)
     {
       const uint4* src = (const uint4*)((const uint16_t*)a.k + b * a.k_seq + (int64_t)key * a.k_tok + h * a.k_head);
 #pragma unroll
       for (int p = 0; p < NP; p++) {
+        if (p != half) continue;
         uint32_t r[32];
 #pragma unroll
         for (int x = 0; x < 8; x++) {
@@ -352,55 +378,49 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
           if (key < a.cache && (8 * p + x) * 8 < a.hd) v = src[8 * p + x];
           r[4 * x] = v.x, r[4 * x + 1] = v.y, r[4 * x + 2] = v.z, r[4 * x + 3] = v.w;
         }
-        dcu::st32(lane_at + k_col(g) + 32 * p, r);
+        dcu::st32(lane_at + 32 * p, r);
       }
       dcu::wait_st();
       dcu::fence_before();
       __syncwarp();
-      if (lane == 0) dcp::mbar_arrive(&s_free[g]);
+      if (lane == 0) dcp::mbar_arrive(k_ready);
     }
-    const int64_t lse_at = (int64_t)b * a.rows * a.heads + h * a.group;
-    float* L2 = scales + g * 2 * COLS;
-    float next = lse_of(a, lse_at, t0, me), sum = 0.0f;
-    bool ok = true;  // (a warp whose wait gave up stays in the loop: the others count on it at the barrier)
-    for (int i = 0; i < n; i++) {
-      float* L = L2 + (i & 1) * COLS;
-      L[me] = scale_of(next);
-      if (i + 1 < n) next = lse_of(a, lse_at, t0 + i + 1, me);  // (used a tile later)
-      // (one barrier a tile: who passes it has read the buffer of two tiles ago)
-      dcp::named_sync(1 + g, 128);
-      ok = ok && dcu::warp_wait(&s_full[g], i & 1, a.status);
-      if (!ok) continue;
-      dcu::fence_after();
-      const int first_row = (t0 + i) * a.tile_rows;
-      const int from = a.causal ? max(0, key - len + a.rows - first_row) * a.group : 0;  // columns that see the key
-      const int cols = min(a.tile_cols, (a.rows - first_row) * a.group);
-      const bool late = __any_sync(~0u, from > 0);
-      F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
+    const int hidden = a.causal ? key - len + a.rows : 0;  // rows that do not see the key
+    float sum = 0.0f;
+    bool ok = true;
 #pragma unroll 1
-      for (int c0 = 0; c0 < COLS; c0 += 64) {
-        uint32_t x[32], y[32];
-        dcu::ld32(lane_at + s_col(g) + c0, x);
-        dcu::ld32(lane_at + s_col(g) + c0 + 32, y);
-        dcu::wait_ld(x);
-        dcu::wait_ld(y);
-        if (c0 == 64) {
-          // the next tile's products run under the rest of this one's exponentials
-          dcu::fence_before();
-          __syncwarp();
-          if (lane == 0) dcp::mbar_arrive(&s_free[g]);
-        }
-        if (c0 < cols) add_columns<MANY_EVERY>(part, x, L, a.c, c0, from, cols, late);
-        if (c0 + 32 < cols) add_columns<MANY_EVERY>(part, y, L, a.c, c0 + 32, from, cols, late);
-      }
+    for (int u = 0; u < 2 * n; u++) {
+      const int i = u >> 1, st = i % SCALES, buf = u % BUFS;
+      const bool odd = lane & 1;
+      ok = dcu::warp_wait(odd ? &l_full[st] : &s_full[buf], odd ? (i / SCALES) & 1 : (u / BUFS) & 1, a.status);
+      if (!ok) break;
+      dcu::fence_after();
+      const int first_row = (t0 + i) * a.tile_rows, c0 = (u & 1) * HALF + half * 32;
+      const int cols = min(a.tile_cols, (a.rows - first_row) * a.group);
+      const bool late = __any_sync(~0u, hidden > first_row);
+      const int from = late ? max(0, hidden - first_row) * a.group : 0;  // columns that see the key
+      F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
+      const float* L = scales + st * COLS;
+      uint32_t x[32];
+      dcu::ld32(lane_at + s_col(buf) + half * 32, x);
+      dcu::wait_ld(x);
+      dcu::fence_before();
+      __syncwarp();
+      if (lane == 0) dcp::mbar_arrive(&s_free[buf]);
+      if (c0 < cols) add_columns<MANY_EVERY>(part, x, L, a.c, c0, from, cols, late);
       sum += sum_of(part);
+      __syncwarp();
+      if ((u & 1) && lane == 0) dcp::mbar_arrive(&l_free[st]);
     }
-    if (ok && key < len) put(a, b, h, key, sum);
+    if (half) halves[quarter * 32 + lane] = ok ? sum : -1.0f;
+    dcp::named_sync(1, 256);
+    const float other = halves[quarter * 32 + lane];
+    if (!half && ok && key < len && other != -1.0f) put(a, b, h, key, sum + other);
   }
   __syncthreads();
   if (warp == MMA_WARP) {
     dcu::fence_after();
-    dcu::dealloc(tmem, 512);
+    dcu::dealloc(tmem, 256);
   }
 }
 
@@ -453,8 +473,8 @@ extern "C" int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* p) {
   a.cols_mma = (a.tile_cols + 31) / 32 * 32;  // (columns are read 32 at a time)
   const int64_t heads = (int64_t)A.batch * A.kv_heads, tiles = (A.cache + KEYS - 1) / KEYS;
   // few: one wave of two blocks an SM, each an even share of a head's key
-  // tiles; many: a block for every two key tiles
-  int64_t splits = (tiles + 1) / 2;
+  // tiles; many: a block for every key tile
+  int64_t splits = tiles;
   if (few) {
     splits = std::min(tiles, std::max<int64_t>(1, 2 * (int64_t)ctx->sm_count / heads));
     const int64_t each = (tiles + splits - 1) / splits;
