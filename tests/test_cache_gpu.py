@@ -330,6 +330,68 @@ def test_attention_non_finite_scores(comp):
     assert torch.isnan(out[:, :, 2:]).all() and torch.isnan(lse[:, :, 2:]).all() and (out[0, :, :2] == 0).all()
 
 
+# Row counts around what one tile of rows, two, and the small batches' kernel take; key counts around its
+# tiles of 16 and 64 and the others' of 128: batch, rows, heads, kv, D, prefix, own_max, lens, type, out type
+ATTN_EDGES = [
+    (31, 1, 1, 1, 64, 15, 0, None, BF16, BF16),
+    (32, 1, 2, 2, 64, 16, 3, [3] * 32, F16, F16),
+    (33, 1, 2, 2, 64, 17, 3, [2] * 33, F16, F16),
+    (4, 4, 8, 4, 128, 63, 0, None, F16, F32),
+    (4, 4, 8, 4, 128, 1025, 30, [4, 30, 0, 17], BF16, BF16),
+    (11, 3, 4, 4, 128, 127, 0, None, BF16, BF16),
+    (11, 3, 4, 4, 128, 256, 0, None, BF16, F32),
+    (128, 1, 2, 2, 8, 128, 0, None, F16, F16),
+    (129, 1, 2, 2, 64, 129, 0, None, BF16, BF16),
+    (16, 16, 2, 2, 128, 385, 20, [20] * 16, F16, F16),
+    (257, 1, 1, 1, 120, 130, 0, None, BF16, BF16),
+    (64, 1, 4, 1, 64, 1, 0, None, BF16, BF16),
+]
+
+
+@pytest.mark.parametrize("case", ATTN_EDGES,
+                         ids=lambda c: "x".join(str(v).replace("torch.", "") for v in c[:7]) + str(c[8])[6:])
+def test_prefix_attention_edges(comp, case):
+    test_prefix_attention(comp, case)
+
+
+@pytest.mark.parametrize("B, D, t", [(12, 128, BF16), (12, 64, F16), (40, 128, F16), (40, 64, BF16), (100, 128, BF16)])
+def test_shared_prefix_with_growing_scores(comp, B, D, t):
+    """As above for more rows: one tile of rows whose groups join, pairs of tiles, a pair and one by itself."""
+    g = gen(B + D)
+    H, kv, P = 8, 2, 1500
+    q = torch.ones(B, 1, H, D, device="cuda").to(t) * 0.5
+    kp = (torch.linspace(-30, 60, P, device="cuda").view(P, 1, 1) / D * 2).expand(P, kv, D).to(t)
+    vp = normal(g, P, kv, D).to(t)
+    out, lse = torch.empty_like(q), torch.empty(B, 1, H, device="cuda")
+    comp.prefix_attention_dev(q, out, kp, vp, lse=lse, scale=1.0)
+    comp.sync()
+    check_attention(out, lse, attention_ref(q, kp, vp, None, None, None, 1.0), t, 6.0)
+
+
+@pytest.mark.parametrize("B, D", [(12, 128), (12, 64), (40, 128), (40, 64)])
+def test_shared_prefix_non_finite_scores(comp, B, D):
+    """The same at -inf and NaN: an empty head, one whose later keys take no part, one that is spoiled."""
+    g = gen(B + D + 1)
+    H, kv, P, t = 12, 3, 600, BF16
+    q = normal(g, B, 1, H, D).abs().to(t)
+    kp, vp = normal(g, P, kv, D).to(t), normal(g, P, kv, D).to(t)
+    kp[:, 0] = -math.inf
+    kp[:200, 1] = -math.inf
+    kp[301:, 1] = -math.inf
+    out, lse = torch.empty_like(q), torch.empty(B, 1, H, device="cuda")
+    comp.prefix_attention_dev(q, out, kp, vp, lse=lse)
+    comp.sync()
+    assert (out[:, :, :4] == 0).all() and torch.isneginf(lse[:, :, :4]).all()
+    fine = attention_ref(q[:, :, 4:8], kp[200:301, 1:2], vp[200:301, 1:2], None, None, None, D ** -0.5)
+    check_attention(out[:, :, 4:8], lse[:, :, 4:8], fine, t, 6.0)
+    fine = attention_ref(q[:, :, 8:], kp[:, 2:], vp[:, 2:], None, None, None, D ** -0.5)
+    check_attention(out[:, :, 8:], lse[:, :, 8:], fine, t, 6.0)
+    kp[599, 2, 5] = math.nan
+    comp.prefix_attention_dev(q, out, kp, vp, lse=lse)
+    comp.sync()
+    assert torch.isnan(out[:, :, 8:]).all() and torch.isnan(lse[:, :, 8:]).all() and (out[:, :, :4] == 0).all()
+
+
 def test_attention_equal_inputs_equal_bits(comp):
     g = gen(11)
     q = normal(g, 40, 1, 8, 128).to(BF16)
