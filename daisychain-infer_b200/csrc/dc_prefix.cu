@@ -109,7 +109,9 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // probabilities, store and product, which two groups fill only in part.  Twice the
 // warps a group, rolled loops, the maximum of the tile before, a forced
 // order of the groups and an issuing warp for each kind of product gave nothing or
-// lost; there is no TMEM for a third group.
+// lost; scores of 64 keys, two buffers a group, one being formed under the other's
+// softmax, took 106 us for 64 sequences over 65536 keys where this takes 100 (and 53
+// for 56 on 24 x 5 drafts of 64 channels); there is no TMEM for a third group.
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
 constexpr int SH_THREADS = 384;
