@@ -28,10 +28,12 @@
 // so that k_join, which waits for k_own, finds both complete.
 //
 // Every wait on a barrier is bounded (dc_ptx.cuh); a block whose wait gives up
-// ends, and dc_sync reports it.
+// waits for the copies and products that it has in flight (bounded as well) and ends,
+// its part without weight, and dc_sync reports it.
 #include <algorithm>
 
 #include "dc_cache.cuh"
+#include "dc_ring.h"
 #include "dc_umma.cuh"
 
 namespace {
@@ -125,7 +127,7 @@ struct Shared {
   static constexpr int PANEL = 128 * 128;
   static constexpr int TILE = NP * PANEL;
   static constexpr int STAGES = NP == 2 ? 5 : 8;
-  static constexpr int BARS = 2 * STAGES + 12;
+  static constexpr int BARS = 2 * STAGES + 13;
   static constexpr int SMEM = (2 + STAGES) * TILE + BARS * 8 + 8;  // (and a slot for the TMEM address)
   // TMEM columns of group g: scores, O, probabilities
   static constexpr bool APART = NP == 1;  // probabilities beside the scores
@@ -154,6 +156,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
   uint64_t* p_ready = s_free + 2;        // [2 x 2] half of its probabilities are in TMEM
   uint64_t* o_done = p_ready + 4;        // [2] its O holds the tile
   uint64_t* q_ready = o_done + 2;        // [2]
+  uint64_t* idle = q_ready + 2;          // all products that were issued are complete
   uint32_t* slot = (uint32_t*)(full + C::BARS);
 
   const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -183,6 +186,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
       dcp::mbar_init(&o_done[i], 1);
       dcp::mbar_init(&q_ready[i], 4);
     }
+    dcp::mbar_init(idle, 1);
     dcp::mbar_fence_init();
   }
   if (warp == MMA_WARP) dcu::alloc(slot, 512);
@@ -214,10 +218,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           dcu::tma_load_3d(ring + st * C::TILE + p * C::PANEL, is_k ? &map_k : &map_v, p * 64, h, k0 + tile * KEYS,
                            &full[st]);
       }
-      // (given up: what is in flight lands before the block's memory goes away)
-      if (issued < 2 * n)
-        for (int s = max(0, issued - C::STAGES); s < issued; s++)
-          dcp::mbar_wait(&full[s % C::STAGES], (s / C::STAGES) & 1, a.status);
+      dcr::drain<C::STAGES>(issued, [&](int st, uint32_t par) { dcp::mbar_wait(&full[st], par, a.status); });
     }
   } else if (warp == MMA_WARP) {
     // ---- products, of the groups by turns: that keeps their softmaxes half a
@@ -274,6 +275,10 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
         if (!C::APART && ok && j + 1 < count) ok = scores(g, j + 1);
       }
     }
+    // (also where a wait gave up: nothing reads the ring or writes TMEM any more)
+    if (dcu::elect()) dcu::commit(idle);
+    __syncwarp();
+    dcu::warp_wait(idle, 0, a.status);
   } else if (warp >= EXP_WARP) {
     const int g = (warp - EXP_WARP) >> 2, quarter = warp & 3;  // group, TMEM lanes
     const int m = 2 * pair + (two ? g : 0);
@@ -614,12 +619,11 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
     for (int x = 0; x < 8 * NP; x++)
 #pragma unroll
       for (int y = 0; y < 4; y++) o[x][y] = 0.0f;
-    bool ok = true;
+    int i = 0;
     const int key_k = (lane / 16) * 8 + lane % 8, key_v = ((lane / 8) & 1) * 8 + lane % 8;
-    for (int i = 0; i < n; i++) {
+    for (; i < n; i++) {
       const int st = i % OWN_STAGES;
-      ok = dcu::warp_wait(&full[st], (i / OWN_STAGES) & 1, a.status);
-      if (!ok) break;
+      if (!dcu::warp_wait(&full[st], (i / OWN_STAGES) & 1, a.status)) break;
       const int nv = min(OWN_KEYS, k1 - key_of(i));
       const uint32_t k_at = dcp::smem_u32(ring + st * 2 * C::TILE), v_at = k_at + C::TILE;
       float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -693,9 +697,11 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
       __syncwarp();
       if (lane == 0 && i + OWN_STAGES < n) copy(i + OWN_STAGES);
     }
-    if (!ok)  // (given up: what is in flight lands before the block's memory goes away)
-      for (int i = 0; i < OWN_STAGES; i++)
-        if (i < n) dcp::mbar_wait(&full[i], 0, a.status);
+    if (i < n) {  // (given up)
+      dcr::drain_own<OWN_STAGES>(i, n, [&](int st, uint32_t par) { dcp::mbar_wait(&full[st], par, a.status); });
+#pragma unroll
+      for (int y = 0; y < 2; y++) mx[y] = -INFINITY, l[y] = 0.0f;
+    }
     // ---- the warps' results
     float* mine = (float*)ring;  // 16 rows of WIDTH + 4 floats (the rows of a fragment in different banks)
 #pragma unroll

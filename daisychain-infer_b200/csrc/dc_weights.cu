@@ -24,10 +24,12 @@
 // a block and two groups of four warps 228.
 //
 // One warp copies, one issues the products.  Every wait is bounded; a block whose
-// wait gives up ends, and dc_sync reports it.
+// wait gives up waits for the copies and products that it has in flight (bounded as
+// well) and ends, and dc_sync reports it.
 #include <algorithm>
 
 #include "dc_cache.cuh"
+#include "dc_ring.h"
 #include "dc_umma.cuh"
 
 namespace {
@@ -43,8 +45,9 @@ constexpr int PANEL_BYTES = 128 * 128;
 constexpr float LOG2E = 1.4426950408889634f;
 
 constexpr int STAGES = 5;  // two blocks an SM hold at most 113 KB each
+constexpr int FEW_BARS = 2 * STAGES + 6;
 template <int NP>
-constexpr int FEW_SMEM = (NP + STAGES) * PANEL_BYTES + COLS * 4 + 128;
+constexpr int FEW_SMEM = (NP + STAGES) * PANEL_BYTES + COLS * 4 + FEW_BARS * 8 + 8;  // (and a slot for the TMEM address)
 
 struct CwArgs {
   const void* k;
@@ -134,7 +137,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   uint64_t* s_full = empty + STAGES;  // [2] scores of a buffer are in TMEM
   uint64_t* s_free = s_full + 2;      // [2] and have been read
   uint64_t* kept_full = s_free + 2;
-  uint32_t* slot = (uint32_t*)(kept_full + 1);
+  uint64_t* idle = kept_full + 1;  // all products that were issued are complete
+  uint32_t* slot = (uint32_t*)(full + FEW_BARS);
 
   const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -155,6 +159,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       dcp::mbar_init(&s_free[i], 4);
     }
     dcp::mbar_init(kept_full, 1);
+    dcp::mbar_init(idle, 1);
     dcp::mbar_fence_init();
   }
   if (warp == 5) dcu::alloc(slot, 2 * COLS);
@@ -180,12 +185,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         dcp::mbar_expect_tx(&full[st], PANEL_BYTES);
         dcu::tma_load_4d(ring + st * PANEL_BYTES, &map_k, p * 64, h, k0 + i * KEYS, b, &full[st]);
       }
-      if (issued < n * NP) {
-        // (given up: what is in flight lands before the block's memory goes away)
-        dcp::mbar_wait(kept_full, 0, a.status);
-        for (int s = max(0, issued - STAGES); s < issued; s++)
-          dcp::mbar_wait(&full[s % STAGES], (s / STAGES) & 1, a.status);
-      }
+      dcp::mbar_wait(kept_full, 0, a.status);
+      dcr::drain<STAGES>(issued, [&](int st, uint32_t par) { dcp::mbar_wait(&full[st], par, a.status); });
     }
   } else if (warp == 5) {
     const uint32_t id = dcu::idesc(BF16, 0, false) | ((uint32_t)(a.cols_mma >> 3) << 17);
@@ -210,6 +211,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         __syncwarp();
       }
     }
+    // (also where a wait gave up: nothing reads shared memory or writes TMEM any more)
+    if (dcu::elect()) dcu::commit(idle);
+    __syncwarp();
+    dcu::warp_wait(idle, 0, a.status);
   } else {
     const uint32_t lane_at = tmem + ((uint32_t)(warp * 32) << 16);
     const int cols = a.tile_cols;
@@ -251,7 +256,7 @@ template <int NP>
 struct Many {
   static constexpr int TILE = NP * PANEL_BYTES;
   static constexpr int STAGES = NP == 2 ? 3 : 6;
-  static constexpr int BARS = 2 * STAGES + 2 * BUFS + 2 * SCALES + 1;
+  static constexpr int BARS = 2 * STAGES + 2 * BUFS + 2 * SCALES + 2;
   static constexpr int SMEM = STAGES * TILE + SCALES * COLS * 4 + KEYS * 4 + BARS * 8 + 8;
 };
 
@@ -270,6 +275,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
   uint64_t* l_full = s_free + BUFS;      // [SCALES] a tile's scales are there
   uint64_t* l_free = l_full + SCALES;    // [SCALES] and have been read
   uint64_t* k_ready = l_free + SCALES;   // the keys are in TMEM
+  uint64_t* idle = k_ready + 1;          // all products that were issued are complete
   uint32_t* slot = (uint32_t*)(full + C::BARS);
 
   const int warp = dcu::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -296,6 +302,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
       dcp::mbar_init(&l_free[i], 8);
     }
     dcp::mbar_init(k_ready, 8);
+    dcp::mbar_init(idle, 1);
     dcp::mbar_fence_init();
   }
   if (warp == MMA_WARP) dcu::alloc(slot, 256);
@@ -318,10 +325,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
         for (int p = 0; p < NP; p++)
           dcu::tma_load_5d(ring + st * C::TILE + p * PANEL_BYTES, &map_q, p * 64, 0, h, (t0 + i) * a.tile_rows, b, &full[st]);
       }
-      // (given up: what is in flight lands before the block's memory goes away)
-      if (issued < n)
-        for (int i = max(0, issued - C::STAGES); i < issued; i++)
-          dcp::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, a.status);
+      dcr::drain<C::STAGES>(issued, [&](int st, uint32_t par) { dcp::mbar_wait(&full[st], par, a.status); });
     }
   } else if (warp == MMA_WARP) {
     const uint32_t id = dcu::idesc(BF16, HALF, false);
@@ -344,6 +348,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
       }
       __syncwarp();
     }
+    // (also where a wait gave up: nothing reads shared memory or writes TMEM any more)
+    if (dcu::elect()) dcu::commit(idle);
+    __syncwarp();
+    dcu::warp_wait(idle, 0, a.status);
   } else if (warp == SCALE_WARP) {
     // ---- each Q tile's scales, a tile's lse read while the one before is waited for
     const int64_t lse_at = (int64_t)b * a.rows * a.heads + h * a.group;
