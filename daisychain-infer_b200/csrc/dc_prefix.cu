@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // A wait of a whole warp for two barriers at once.
 __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py, int* status) {
   const bool odd = threadIdx.x & 1;
-  return dcu::warp_wait(odd ? y : x, odd ? py : px, status);
+  return dcu::warp_wait_each(odd ? y : x, odd ? py : px, status);
 }
 
 // ---- the shared prefix ----------------------------------------------------------

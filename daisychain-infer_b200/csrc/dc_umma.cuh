@@ -84,6 +84,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
       : "memory");
   return __all_sync(~0u, met) || __all_sync(~0u, dcp::mbar_wait(bar, parity, status));
 }
+// The same where the lanes wait for different barriers, and all go on to use what any
+// of them guards: a vote orders no memory between lanes, __syncwarp does.
+__device__ __forceinline__ bool warp_wait_each(uint64_t* bar, uint32_t parity, int* status) {
+  const bool met = warp_wait(bar, parity, status);
+  __syncwarp();
+  return met;
+}
 // D (TMEM) (+)= A (shared) x B (shared)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
       const int i = u >> 1, st = i % C::STAGES, buf = u % BUFS;
       // (lanes by turns: the tile is here, the scores before have been read)
       const bool odd = (lane & 1) && u >= BUFS;
-      ok = dcu::warp_wait(odd ? &s_free[buf] : &full[st], odd ? (u / BUFS - 1) & 1 : (i / C::STAGES) & 1, a.status);
+      ok = dcu::warp_wait_each(odd ? &s_free[buf] : &full[st], odd ? (u / BUFS - 1) & 1 : (i / C::STAGES) & 1, a.status);
       if (!ok) break;
       dcu::fence_after();
       if (dcu::elect()) {
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
     for (int u = 0; u < 2 * n; u++) {
       const int i = u >> 1, st = i % SCALES, buf = u % BUFS;
       const bool odd = lane & 1;
-      ok = dcu::warp_wait(odd ? &l_full[st] : &s_full[buf], odd ? (i / SCALES) & 1 : (u / BUFS) & 1, a.status);
+      ok = dcu::warp_wait_each(odd ? &l_full[st] : &s_full[buf], odd ? (i / SCALES) & 1 : (u / BUFS) & 1, a.status);
       if (!ok) break;
       dcu::fence_after();
       const int first_row = (t0 + i) * a.tile_rows, c0 = (u & 1) * HALF + half * 32;

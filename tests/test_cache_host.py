@@ -36,3 +36,13 @@ def test_kernels_drain_before_they_end(name, copiers, own):
     assert len(re.findall(r"\bdcr::drain<", src)) == copiers and len(re.findall(r"\bdcr::drain_own<", src)) == own
     assert len(re.findall(r"commit\(idle\);\s*__syncwarp\(\);\s*dcu::warp_wait\(idle, 0, a\.status\);", src)) == copiers
     assert not re.search(r"if \(issued < ", src)
+
+
+@pytest.mark.parametrize("name, waits", [("dc_prefix.cu", 1), ("dc_weights.cu", 2)])
+def test_lanes_that_wait_for_different_barriers_are_ordered(name, waits):
+    """A vote tells a warp that all its waits are met but orders no memory between its lanes: waits whose
+    lanes look at different barriers end in __syncwarp."""
+    src = source(name)
+    assert len(re.findall(r"\bwarp_wait_each\(odd \?", src)) == waits and not re.search(r"\bwarp_wait\(odd \?", src)
+    body = re.search(r"bool warp_wait_each\(.*?\n}", source("dc_umma.cuh"), re.S).group(0)
+    assert re.search(r"warp_wait\(bar, parity, status\);\s*__syncwarp\(\);\s*return", body)
