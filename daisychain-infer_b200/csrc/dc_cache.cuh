@@ -1,13 +1,11 @@
-// dc_cache.cuh -- what the cache operators share: types, spans of strided
-// buffers (argument checks) and the launch.
+// dc_cache.cuh -- what the cache operators share: types and the launch.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <initializer_list>
-
 #include "dc_internal.cuh"
 #include "dc_ptx.cuh"
+#include "dc_span.h"
 
 namespace dcc {
 
@@ -26,40 +24,6 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// The addresses that a strided buffer covers, from its first to behind its
-// last byte, for the overlap checks.
-struct Dim {
-  int64_t n, stride;
-};
-struct Span {
-  uintptr_t lo = 0, hi = 0;
-  bool ok = true;
-  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
-};
-static inline Span span(const void* p, int elem, std::initializer_list<Dim> dims) {
-  Span s;
-  if (!p) return s;
-  int64_t last = 0;
-  bool empty = false;
-  for (const Dim& d : dims) {
-    if (d.stride < 0) s.ok = false;
-    if (d.n <= 0) empty = true;
-    else last += (d.n - 1) * d.stride;
-  }
-  if (empty || !s.ok) return s;
-  s.lo = (uintptr_t)p;
-  s.hi = s.lo + (uintptr_t)(last + 1) * elem;
-  return s;
-}
-// Whether a buffer of es-byte elements begins, and each of its rows in these
-// dimensions, on a boundary of `align` bytes.
-static inline bool aligned(const void* p, int es, int align, std::initializer_list<Dim> dims) {
-  uintptr_t m = (uintptr_t)p;
-  for (const Dim& d : dims)
-    if (d.n > 1) m |= (uintptr_t)(d.stride * es);
-  return !(m & (align - 1));
-}
 
 // A call may come while another device is current: launches and kernel
 // attributes belong to the context's own.

@@ -317,20 +317,25 @@ extern "C" int dc_cache_evict_dev(dc_ctx* ctx, const dc_cache_evict* p) {
       span(A.k, es, {{A.batch, A.k_seq}, {A.cache, A.k_tok}, {A.kv_heads, A.k_head}, {A.head_dim, 1}}),
       span(A.v, es, {{A.batch, A.v_seq}, {A.cache, A.v_tok}, {A.kv_heads, A.v_head}, {A.head_dim, 1}}),
       span(A.acc, 4, {{A.batch, A.acc_seq}, {A.kv_heads, A.acc_head}, {A.cache, 1}}), span(A.lens, 4, {{A.batch, 1}})};
-  const Span out[5] = {
-      span(A.k_out, es, {{A.batch, A.ko_seq}, {most, A.ko_tok}, {A.kv_heads, A.ko_head}, {A.head_dim, 1}}),
-      span(A.v_out, es, {{A.batch, A.vo_seq}, {most, A.vo_tok}, {A.kv_heads, A.vo_head}, {A.head_dim, 1}}),
-      span(A.acc_out, 4, {{A.batch, A.acco_seq}, {A.kv_heads, A.acco_head}, {most, 1}}),
-      span(A.index, 4, {{A.batch, A.idx_seq}, {A.kv_heads, A.idx_head}, {most, 1}}), span(A.lens_out, 4, {{A.batch, 1}})};
+  const std::initializer_list<Dim> dk = {
+      {A.batch, A.ko_seq}, {most, A.ko_tok}, {A.kv_heads, A.ko_head}, {A.head_dim, 1}};
+  const std::initializer_list<Dim> dv = {
+      {A.batch, A.vo_seq}, {most, A.vo_tok}, {A.kv_heads, A.vo_head}, {A.head_dim, 1}};
+  const std::initializer_list<Dim> da = {{A.batch, A.acco_seq}, {A.kv_heads, A.acco_head}, {most, 1}};
+  const std::initializer_list<Dim> di = {{A.batch, A.idx_seq}, {A.kv_heads, A.idx_head}, {most, 1}};
+  const Span out[5] = {span(A.k_out, es, dk), span(A.v_out, es, dv), span(A.acc_out, 4, da), span(A.index, 4, di),
+                       span(A.lens_out, 4, {{A.batch, 1}})};
   for (const Span& o : out) {
     for (const Span& i : in)
       if (!o.ok || !i.ok || o.meets(i))
         return dc_fail(ctx, DC_E_INVAL, "cache_evict: a negative stride, or an output overlaps an input");
-    // (k_out and v_out may be interleaved in one buffer, so only the same address is refused there)
+    // (k_out and v_out may be interleaved in one buffer)
     for (const Span& q : out)
-      if (&q < &o && o.meets(q) && !(&o == &out[1] && &q == &out[0] && o.lo != q.lo))
+      if (&q < &o && !(&o == &out[1] && &q == &out[0] ? twins_apart(q, o, es, dk, dv) : !o.meets(q)))
         return dc_fail(ctx, DC_E_INVAL, "cache_evict: two outputs overlap");
   }
+  if (!apart(dk) || !apart(dv) || !apart(da) || !apart(di))
+    return dc_fail(ctx, DC_E_INVAL, "cache_evict: two elements of an output share an address");
   DeviceGuard guard;
   if (int rc = guard.enter(ctx)) return rc;
 

@@ -1015,7 +1015,9 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
     return dc_fail(ctx, DC_E_INVAL, "prefix_attention: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes,
                    need);
   const Span q = span(A.q, 2, {{A.batch, A.q_seq}, {A.rows, A.q_row}, {A.heads, A.q_head}, {A.head_dim, 1}});
-  const Span o = span(A.out, es_o, {{A.batch, A.out_seq}, {A.rows, A.out_row}, {A.heads, A.out_head}, {A.head_dim, 1}});
+  const std::initializer_list<Dim> d_out = {
+      {A.batch, A.out_seq}, {A.rows, A.out_row}, {A.heads, A.out_head}, {A.head_dim, 1}};
+  const Span o = span(A.out, es_o, d_out);
   const Span l = span(A.lse, 4, {{(int64_t)A.batch * A.rows * A.heads, 1}});
   const Span w = span(need ? ws : nullptr, 1, {{(int64_t)need, 1}});
   const Span n = span(A.own_max ? A.lens : nullptr, 4, {{A.batch, 1}});
@@ -1033,6 +1035,7 @@ extern "C" int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* p, voi
     over |= o.meets(s) || l.meets(s) || w.meets(s);
   }
   if (bad) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: negative stride");
+  if (!apart(d_out)) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: two elements of out share an address");
   if (over) return dc_fail(ctx, DC_E_INVAL, "prefix_attention: out, lse or ws overlaps another buffer");
   DeviceGuard guard;
   if (int rc = guard.enter(ctx)) return rc;

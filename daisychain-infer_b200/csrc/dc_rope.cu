@@ -309,14 +309,18 @@ extern "C" int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* p) {
                    (long long)A.cache_seqs, (long long)A.cache_len);
   const int es_i = elem_size(A.x_type), es_o = elem_size(A.out_type);
   const Span x = span(A.x, es_i, {{A.rows, A.ldx}, {width, 1}});
-  const Span q = span(A.heads ? A.q : nullptr, es_o, {{A.rows, A.q_row}, {A.heads, A.q_head}, {A.head_dim, 1}});
-  const Span k = span(A.kv_heads ? A.k : nullptr, es_o,
-                      {{A.cache_seqs, A.k_seq}, {A.cache_len, A.k_tok}, {A.kv_heads, A.k_head}, {A.head_dim, 1}});
-  const Span v = span(A.kv_heads ? A.v : nullptr, es_o,
-                      {{A.cache_seqs, A.v_seq}, {A.cache_len, A.v_tok}, {A.kv_heads, A.v_head}, {A.head_dim, 1}});
+  const std::initializer_list<Dim> dq = {{A.rows, A.q_row}, {A.heads, A.q_head}, {A.head_dim, 1}};
+  const std::initializer_list<Dim> dk = {
+      {A.cache_seqs, A.k_seq}, {A.cache_len, A.k_tok}, {A.kv_heads, A.k_head}, {A.head_dim, 1}};
+  const std::initializer_list<Dim> dv = {
+      {A.cache_seqs, A.v_seq}, {A.cache_len, A.v_tok}, {A.kv_heads, A.v_head}, {A.head_dim, 1}};
+  const Span q = span(A.heads ? A.q : nullptr, es_o, dq), k = span(A.kv_heads ? A.k : nullptr, es_o, dk),
+             v = span(A.kv_heads ? A.v : nullptr, es_o, dv);
   if (!q.ok || !k.ok || !v.ok) return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: negative stride");
-  // (k and v may be interleaved in one buffer, so only the same address is refused)
-  if (x.meets(q) || x.meets(k) || x.meets(v) || q.meets(k) || q.meets(v) || (k.hi && k.lo == v.lo))
+  if (!apart(dq) || !apart(dk) || !apart(dv))
+    return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: two elements of q, k or v share an address");
+  // (k and v may be interleaved in one buffer)
+  if (x.meets(q) || x.meets(k) || x.meets(v) || q.meets(k) || q.meets(v) || !twins_apart(k, v, es_o, dk, dv))
     return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: an output overlaps x or another output");
   DeviceGuard g;
   if (int rc = g.enter(ctx)) return rc;

@@ -461,13 +461,15 @@ extern "C" int dc_cache_weights_dev(dc_ctx* ctx, const dc_cache_weight* p) {
   if (!aligned(A.q, 2, 16, {{A.batch, A.q_seq}, {A.rows, A.q_row}, {A.heads, A.q_head}}) ||
       !aligned(A.k, 2, 16, {{A.batch, A.k_seq}, {A.cache, A.k_tok}, {A.kv_heads, A.k_head}}))
     return dc_fail(ctx, DC_E_INVAL, "cache_weights: q and k rows must begin on 16-byte boundaries");
-  const Span acc = span(A.acc, 4, {{A.batch, A.acc_seq}, {A.kv_heads, A.acc_head}, {A.cache, 1}});
+  const std::initializer_list<Dim> d_acc = {{A.batch, A.acc_seq}, {A.kv_heads, A.acc_head}, {A.cache, 1}};
+  const Span acc = span(A.acc, 4, d_acc);
   const Span in[4] = {span(A.q, 2, {{A.batch, A.q_seq}, {A.rows, A.q_row}, {A.heads, A.q_head}, {A.head_dim, 1}}),
                       span(A.k, 2, {{A.batch, A.k_seq}, {A.cache, A.k_tok}, {A.kv_heads, A.k_head}, {A.head_dim, 1}}),
                       span(A.lse, 4, {{(int64_t)A.batch * A.rows * A.heads, 1}}), span(A.lens, 4, {{A.batch, 1}})};
   for (const Span& s : in)
     if (!acc.ok || !s.ok || acc.meets(s))
       return dc_fail(ctx, DC_E_INVAL, "cache_weights: a negative stride, or acc overlaps an input");
+  if (!apart(d_acc)) return dc_fail(ctx, DC_E_INVAL, "cache_weights: two elements of acc share an address");
   DeviceGuard guard;
   if (int rc = guard.enter(ctx)) return rc;
 

@@ -188,7 +188,9 @@ int dc_rmsnorm_dev(dc_ctx* ctx, const float* x, int rows, int cols, const float*
  * Types are DC_F32 / DC_F16 / DC_BF16; strides are in elements, the last
  * dimension (head_dim) is contiguous.  All calls are asynchronous on the
  * context's stream, allocate nothing, and may be captured into a graph.  A buffer
- * that a call writes lies apart from those it reads and writes besides. */
+ * that a call writes lies apart from those it reads and writes besides, and no two
+ * of its elements share an address (keys and values may be interleaved in one
+ * buffer, with equal strides). */
 #define DC_F32 0
 #define DC_F16 1
 #define DC_BF16 2

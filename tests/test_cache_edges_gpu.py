@@ -1,0 +1,44 @@
+"""The cache operators at the ends of what their arguments may hold, against 64 bits."""
+import pytest
+import torch
+
+from test_cache_gpu import F32, z
+
+pytestmark = pytest.mark.gpu
+
+
+def test_outputs_that_overlap_themselves_are_refused(P, comp):
+    """Expanded outputs, and values a token behind their keys: refused before anything is launched.  Interleaved
+    and permuted ones are taken."""
+    before = comp.L.dc_launch_count()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def refused(call, match):
+        with pytest.raises(P.DeviceError, match=match):
+            call()
+
+    r = dict(x=z(2, 64 * 4, t=F32), pos=i32(0, 1), q=z(2, 2, 64), k=z(2, 1, 64), v=z(2, 1, 64))
+    for name in ("q", "k", "v"):
+        refused(lambda: comp.head_norm_rope_dev(**{**r, name: r[name][:1].expand_as(r[name])}), "share an address")
+    line = z(3, 1, 64)
+    refused(lambda: comp.head_norm_rope_dev(**{**r, "k": line[:2], "v": line[1:]}), "overlaps")
+
+    a = dict(q=z(2, 1, 4, 64), k_pre=z(5, 2, 64), v_pre=z(5, 2, 64))
+    refused(lambda: comp.prefix_attention_dev(out=z(1, 1, 4, 64).expand(2, 1, 4, 64), **a), "share an address")
+    refused(lambda: comp.prefix_attention_dev(out=z(2, 1, 1, 64).expand(2, 1, 4, 64), **a), "share an address")
+
+    w = dict(q=z(2, 1, 4, 64), k=z(2, 5, 2, 64), lens=i32(5, 5), lse=z(2, 1, 4, t=F32))
+    refused(lambda: comp.cache_weights_dev(acc=z(2, 1, 5, t=F32).expand(2, 2, 5), **w), "share an address")
+    refused(lambda: comp.cache_weights_dev(acc=z(1, 2, 5, t=F32).expand(2, 2, 5), **w), "share an address")
+    refused(lambda: comp.cache_weights_dev(acc=z(24, t=F32).as_strided((2, 2, 5), (10, 4, 1)), **w), "share an address")
+
+    e = dict(k=z(2, 9, 2, 64), v=z(2, 9, 2, 64), acc=z(2, 2, 9, t=F32), lens=i32(9, 9), k_out=z(2, 4, 2, 64),
+             v_out=z(2, 4, 2, 64), acc_out=z(2, 2, 4, t=F32), index=z(2, 2, 4, t=torch.int32), lens_out=i32(0, 0))
+    for name in ("k_out", "v_out", "acc_out", "index"):
+        refused(lambda: comp.cache_evict_dev(**{**e, name: e[name][:1].expand_as(e[name])}, budget=4), "share an address")
+    line = z(2, 5, 2, 64)
+    refused(lambda: comp.cache_evict_dev(**{**e, "k_out": line[:, :4], "v_out": line[:, 1:]}, budget=4), "overlap")
+    assert comp.L.dc_launch_count() == before
+    comp.cache_evict_dev(**{**e, "k_out": (both := z(2, 4, 2, 2, 64))[:, :, 0], "v_out": both[:, :, 1]}, budget=4)
+    comp.cache_evict_dev(**{**e, "k_out": (both := z(2, 4, 2, 2, 64))[..., 0, :], "v_out": both[..., 1, :]}, budget=4)
+    comp.sync()

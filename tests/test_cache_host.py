@@ -24,6 +24,10 @@ def run(tmp_path):
     return go
 
 
+def test_checks_of_strided_buffers(run):
+    run("span")
+
+
 def test_drained_rings_have_nothing_in_flight(run):
     run("ring")
 
