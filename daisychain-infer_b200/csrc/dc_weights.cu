@@ -47,7 +47,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int STAGES = 5;  // two blocks an SM hold at most 113 KB each
 constexpr int FEW_BARS = 2 * STAGES + 6;
 template <int NP>
-constexpr int FEW_SMEM = (NP + STAGES) * PANEL_BYTES + COLS * 4 + FEW_BARS * 8 + 8;  // (and a slot for the TMEM address)
+constexpr int FEW_SMEM = (NP + STAGES) * PANEL_BYTES + COLS * 4 + COLS / 8 + FEW_BARS * 8 + 8;  // (and a slot for the TMEM address)
 
 struct CwArgs {
   const void* k;
@@ -63,17 +63,26 @@ struct CwArgs {
   int* status;
 };
 
-// The exponentials of 32 columns c0.. of a tile (scores x, scales L) added to
-// `part`: those from column `from` up to `cols`.  Every `every`-th pair is taken on the
-// multiply-add pipe.
+// Of 32 columns from c0, a bit for each that is not summed: before `from` (they do not
+// see the key), from `cols` on, and those in `gaps`.
+__device__ __forceinline__ uint32_t left_out(int c0, int from, int cols, uint32_t gaps) {
+  if (from > c0) gaps |= from - c0 >= 32 ? ~0u : (1u << (from - c0)) - 1;
+  if (cols < c0 + 32) gaps |= cols <= c0 ? ~0u : ~0u << (cols - c0);
+  return gaps;
+}
+// The exponentials of columns c0.. + 31 of a tile (scores x, scales L) added to `part`,
+// but for those left out: their scores may be anything, and NaN - inf is not -inf.
+// `late`: a lane of the warp has a `from` above 0.  Every `EVERY`-th pair is taken on
+// the multiply-add pipe.
 template <int EVERY>
 __device__ __forceinline__ void add_columns(F2 (&part)[4], const uint32_t (&x)[32], const float* L, float c, int c0,
-                                            int from, int cols, bool late) {
-  if (late || c0 + 32 > cols) {
+                                            int from, int cols, bool late, uint32_t gaps) {
+  if (late || gaps || c0 + 32 > cols) {
+    const uint32_t out = left_out(c0, from, cols, gaps);
 #pragma unroll
     for (int j = 0; j < 32; j++) {
       const float e = dcu::ex2(fmaf(__uint_as_float(x[j]), c, L[c0 + j]));
-      part[j & 3] = dcu::add2(part[j & 3], dcu::f2(c0 + j < from || c0 + j >= cols ? 0.0f : e, 0.0f));
+      part[j & 3] = dcu::add2(part[j & 3], dcu::f2(out & (1u << j) ? 0.0f : e, 0.0f));
     }
     return;
   }
@@ -132,7 +141,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   uint8_t* kept = smem;
   uint8_t* ring = smem + NP * PANEL_BYTES;
   float* L = (float*)(ring + STAGES * PANEL_BYTES);  // the columns' scales
-  uint64_t* full = (uint64_t*)(L + COLS);
+  uint32_t* gaps = (uint32_t*)(L + COLS);            // a bit for each column of lse -inf
+  uint64_t* full = (uint64_t*)(gaps + COLS / 32);
   uint64_t* empty = full + STAGES;
   uint64_t* s_full = empty + STAGES;  // [2] scores of a buffer are in TMEM
   uint64_t* s_free = s_full + 2;      // [2] and have been read
@@ -164,8 +174,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   }
   if (warp == 5) dcu::alloc(slot, 2 * COLS);
   zero_rows(kept, NP, a.tile_cols, FEW_THREADS);
-  if (threadIdx.x < COLS) L[threadIdx.x] = scale_of(lse_of(a, (int64_t)b * a.rows * a.heads + h * a.group, 0, threadIdx.x));
+  float lse = INFINITY;
+  if (threadIdx.x < COLS) {
+    lse = lse_of(a, (int64_t)b * a.rows * a.heads + h * a.group, 0, threadIdx.x);
+    L[threadIdx.x] = scale_of(lse);
+  }
   dcu::fence_before();
+  const uint32_t gap = __ballot_sync(~0u, lse == -INFINITY);
+  if (threadIdx.x < COLS && lane == 0) gaps[warp] = gap;
   __syncthreads();
   dcu::fence_after();
   const uint32_t tmem = dcu::uniform(*slot);
@@ -228,9 +244,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
 #pragma unroll 1
       for (int c0 = 0; c0 < cols; c0 += 32) {
         uint32_t x[32];
+        const uint32_t gap = gaps[c0 / 32];
         dcu::ld32(lane_at + (i & 1) * COLS + c0, x);
         dcu::wait_ld(x);
-        add_columns<1 << 20>(part, x, L, a.c, c0, from, cols, late);
+        add_columns<1 << 20>(part, x, L, a.c, c0, from, cols, late, gap);
       }
       dcu::fence_before();
       __syncwarp();
@@ -257,7 +274,7 @@ struct Many {
   static constexpr int TILE = NP * PANEL_BYTES;
   static constexpr int STAGES = NP == 2 ? 3 : 6;
   static constexpr int BARS = 2 * STAGES + 2 * BUFS + 2 * SCALES + 2;
-  static constexpr int SMEM = STAGES * TILE + SCALES * COLS * 4 + KEYS * 4 + BARS * 8 + 8;
+  static constexpr int SMEM = STAGES * TILE + SCALES * COLS * 4 + KEYS * 4 + SCALES * COLS / 8 + BARS * 8 + 8;
 };
 
 template <int NP, bool BF16>
@@ -268,7 +285,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
   uint8_t* ring = smem;
   float* scales = (float*)(ring + C::STAGES * C::TILE);  // [SCALES tiles][COLS]
   float* halves = scales + SCALES * COLS;                // [KEYS] sums of the second warps
-  uint64_t* full = (uint64_t*)(halves + KEYS);
+  uint32_t* gaps = (uint32_t*)(halves + KEYS);           // [SCALES tiles] a bit for each column of lse -inf
+  uint64_t* full = (uint64_t*)(gaps + SCALES * COLS / 32);
   uint64_t* empty = full + C::STAGES;
   uint64_t* s_full = empty + C::STAGES;  // [BUFS] a half tile's scores are in TMEM
   uint64_t* s_free = s_full + BUFS;      // [BUFS] and have been read
@@ -364,6 +382,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
 #pragma unroll
       for (int x = 0; x < COLS / 32; x++) {
         scales[st * COLS + x * 32 + lane] = scale_of(next[x]);
+        const uint32_t gap = __ballot_sync(~0u, next[x] == -INFINITY);
+        if (lane == 0) gaps[st * (COLS / 32) + x] = gap;
         if (i + 1 < n) next[x] = lse_of(a, lse_at, t0 + i + 1, x * 32 + lane);
       }
       __syncwarp();
@@ -409,13 +429,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 2)
       const int from = late ? max(0, hidden - first_row) * a.group : 0;  // columns that see the key
       F2 part[4] = {dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0), dcu::f2(0, 0)};
       const float* L = scales + st * COLS;
+      const uint32_t gap = gaps[st * (COLS / 32) + c0 / 32];
       uint32_t x[32];
       dcu::ld32(lane_at + s_col(buf) + half * 32, x);
       dcu::wait_ld(x);
       dcu::fence_before();
       __syncwarp();
       if (lane == 0) dcp::mbar_arrive(&s_free[buf]);
-      if (c0 < cols) add_columns<MANY_EVERY>(part, x, L, a.c, c0, from, cols, late);
+      if (c0 < cols) add_columns<MANY_EVERY>(part, x, L, a.c, c0, from, cols, late, gap);
       sum += sum_of(part);
       __syncwarp();
       if ((u & 1) && lane == 0) dcp::mbar_arrive(&l_free[st]);

@@ -1,10 +1,34 @@
 """The cache operators at the ends of what their arguments may hold, against 64 bits."""
+import math
+
 import pytest
 import torch
 
-from test_cache_gpu import F32, z
+from test_cache_gpu import BF16, F32, gen, normal, weights_ref, z
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("R, H, kv, D, L, causal", [
+    (4, 8, 2, 64, 300, False), (4, 8, 2, 128, 300, True), (128, 2, 2, 128, 200, False),   # few rows
+    (300, 8, 2, 64, 300, False), (200, 15, 5, 128, 260, True)])                            # many
+def test_weights_of_rows_that_are_left_out(comp, R, H, kv, D, L, causal, bad):
+    """A row of lse -inf adds nothing, whatever its queries hold: a batch's padding is left out that way."""
+    g = gen(R + D)
+    B, t = 2, BF16
+    q, k = normal(g, B, R, H, D).to(t), normal(g, B, L, kv, D).to(t)
+    lse = 1.0 + 3 * torch.rand(B, R, H, generator=g, device="cuda") + math.log(L)
+    out = torch.rand(B, R, H, generator=g, device="cuda") < 0.2
+    out[0, 0, 0] = out[1, R - 1, H - 1] = True
+    lse[out] = -math.inf
+    q[out] = bad
+    acc = torch.rand(B, kv, L, generator=g, device="cuda")
+    before, lens = acc.clone(), [L, L - 70]
+    comp.cache_weights_dev(q, k, torch.tensor(lens, dtype=torch.int32, device="cuda"), lse, acc, decay=0.9, causal=causal)
+    comp.sync()
+    want, tol = weights_ref(torch.where(out.unsqueeze(-1), 0.0, q), k, lens, lse, before, D ** -0.5, 0.9, causal)
+    assert ((acc.double() - want).abs() <= tol).all()
 
 
 def test_outputs_that_overlap_themselves_are_refused(P, comp):
