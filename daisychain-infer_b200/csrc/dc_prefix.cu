@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
     split = t % splits;
     const int bh = t / splits;
     h = bh % a.kv_heads, seq = bh / a.kv_heads;
-    const int seen = max(0, min(a.lens[seq], a.own_max) - (a.rows - 1));  // tokens that all rows see
+    // tokens that all rows see (a length far below 0 is 0 before anything is taken off it)
+    const int seen = max(0, max(0, min(a.lens[seq], a.own_max)) - (a.rows - 1));
     k0 = split * a.own_chunk, k1 = min(seen, k0 + a.own_chunk);
     rows = a.own_rows;
     part = a.own_base + (int64_t)t * rows;

@@ -4,9 +4,26 @@ import math
 import pytest
 import torch
 
-from test_cache_gpu import BF16, F32, gen, normal, weights_ref, z
+from test_cache_gpu import BF16, F32, attention_ref, check_attention, gen, normal, weights_ref, z
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("prefix", [0, 70])
+@pytest.mark.parametrize("R", [1, 4, 16])
+def test_attention_of_the_lowest_lengths(comp, prefix, R):
+    """A length is taken as at least 0, however far below it lies."""
+    g = gen(prefix + R)
+    lens = [-2 ** 31, -2 ** 31 + 1, -2 ** 31 + R - 1, -1, 100]
+    B, H, kv, D, L, t = len(lens), 4, 2, 64, 100, BF16
+    q = normal(g, B, R, H, D).to(t)
+    kp, vp = (normal(g, prefix, kv, D).to(t) if prefix else None for _ in range(2))
+    ko, vo = normal(g, B, L, kv, D).to(t), normal(g, B, L, kv, D).to(t)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(B, R, H, device="cuda")
+    comp.prefix_attention_dev(q, out, kp, vp, ko, vo, ln, lse)
+    comp.sync()
+    check_attention(out, lse, attention_ref(q, kp, vp, ko, vo, lens, D ** -0.5), t, 6.0)
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
