@@ -12,9 +12,12 @@
 //     (and a batch's few rows against the prefix);
 //   * k_join: the parts of a row, and its last tokens (below).
 //
-// A running maximum is raised only when a row's has grown by more than 2^8:
-// until then the row's probabilities stay below 2^8, as exact in either type,
-// and o needs no rescaling.
+// A running maximum is raised only when a row's has grown by more than 2^8; until
+// then o needs no rescaling.  For bf16 the row's probabilities then lie below 2^8, as
+// exact there as below 1.  f16 ends at 2^16 and has no normal numbers below 2^-14, so
+// there they are formed 2^7 larger, up to 2^15: what is lost of a key far below the
+// maximum is at most 2^-32 of it (2^-25 unshifted, and then a few hundred keys 2^-26
+// below a dominant one vanished from out, though not from lse).
 //
 // Rows of one sequence may see different last tokens (rows > 1).  k_own takes
 // only the tokens that all rows see; the up to rows - 1 behind them go to k_join,
@@ -44,6 +47,12 @@ using dcu::F2;
 constexpr int MAX_ROWS = 16;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RAISE = 8.0f;  // growth of a row's maximum (in powers of two) that rescales it
+constexpr float F16_UP = 7.0f;  // powers of two by which f16 probabilities are larger
+// What is taken off a row's exponents where its maximum is mx (a part's m).
+template <bool BF16>
+__device__ __forceinline__ float base_of(float mx, float c) {
+  return fmaf(mx, c, BF16 ? 0.0f : -F16_UP);
+}
 
 struct PaArgs {
   const void *q, *k_own, *v_own;
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           }
           dcu::wait_st();
         }
-        const float base = mx == -INFINITY ? 0.0f : mx * a.c;
+        const float base = mx == -INFINITY ? 0.0f : base_of<BF16>(mx, a.c);
         b2 = dcu::f2(-base, -base);
       }
       bool met = true;
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     uint8_t* mine = ring + (g * 128 + row) * STRIDE;
     ok = ok && count > 0 && used && dcu::warp_wait(&o_done[g], (count - 1) & 1, a.status);
     if (!ok) mx = -INFINITY, l = 0.0f;
-    float2 ml = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, l);
+    float2 ml = make_float2(mx == -INFINITY ? -INFINITY : base_of<BF16>(mx, a.c), l);
     dcp::named_sync(1, 256);
     dcu::fence_after();
     // this row, times f, and (join) the second group's, times f_other; a factor of
@@ -676,7 +685,9 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
             for (int y = 0; y < 4; y++) o[x][y] *= f[y >> 1];
         }
       }
-      const float base[2] = {mx[0] == -INFINITY ? 0.0f : mx[0] * a.c, mx[1] == -INFINITY ? 0.0f : mx[1] * a.c};
+      float base[2];
+#pragma unroll
+      for (int y = 0; y < 2; y++) base[y] = mx[y] == -INFINITY ? 0.0f : base_of<BF16>(mx[y], a.c);
       float e[2][4];
 #pragma unroll
       for (int x = 0; x < 2; x++)
@@ -712,7 +723,7 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
       const int row = lane / 4 + 8 * y;
       if (lane % 4 == 0)
         *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + C::WIDTH) =
-            make_float2(mx[y] == -INFINITY ? -INFINITY : mx[y] * a.c, l[y]);
+            make_float2(mx[y] == -INFINITY ? -INFINITY : base_of<BF16>(mx[y], a.c), l[y]);
 #pragma unroll
       for (int x = 0; x < 8 * NP; x++)
         *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + 8 * x + 2 * (lane % 4)) =

@@ -4,9 +4,39 @@ import math
 import pytest
 import torch
 
-from test_cache_gpu import BF16, F32, attention_ref, check_attention, gen, normal, weights_ref, z
+from test_cache_gpu import BF16, F16, F32, U, attention_ref, check_attention, gen, normal, weights_ref, z
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B, kv", [(4, 2), (60, 2)], ids=["few rows", "shared"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_f16_keeps_what_lies_far_below_the_maximum(comp, B, kv, D):
+    """One key in 16 takes nearly all weight and has the value 0; the others weigh 2^-26 of it and have large values.
+
+    With the exponent shifted so that a row's maximum is 2^7, a probability below f16's normal range is off
+    by half of its smallest step, 2^-25, so by 2^-32 of the maximum: out is off by 2^-32 sum |v| / sum p beside
+    its relative bounds.  (Unshifted, 2^-26 rounds to 0 and the output with it.)"""
+    g = gen(B + D)
+    P, H = 1024, 2 * kv
+    x = torch.zeros(P, device="cuda")
+    x[::16] = 18.015625
+    kp = z(P, kv, D)
+    kp[..., 0] = x.to(F16).view(P, 1)
+    vp = (20000 + 20000 * torch.rand(P, kv, D, generator=g, device="cuda")).to(F16)
+    vp[::16] = 0
+    q = z(B, 1, H, D)
+    q[..., 0] = 1
+    out, lse = torch.empty(B, 1, H, D, device="cuda"), torch.empty(B, 1, H, device="cuda")
+    comp.prefix_attention_dev(q, out, kp, vp, lse=lse, scale=1.0)
+    comp.sync()
+    want, wlse, mag, E, n = attention_ref(q[:1], kp, vp, None, None, None, 1.0)
+    p = torch.exp(x.double() - x.double().max())
+    tol = (U[F16] + E.unsqueeze(-1)) * mag + 2.0 ** -32 * vp.double().sum(0).amax() / p.sum() + 4 * U[F32] * mag
+    assert (tol < 0.1 * want).all()  # (the bound says something)
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), (float(err.max()), float(want.max()))
+    assert ((lse.double() - wlse).abs() <= E + n * U[F32] + 4 * U[F32] * wlse.abs()).all()
 
 
 @pytest.mark.parametrize("prefix", [0, 70])
