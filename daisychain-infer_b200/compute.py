@@ -292,9 +292,13 @@ class Compute:
 
     def prefix_attention_ws(self, q, out, k_pre=None, v_pre=None, k_own=None, v_own=None, lens=None, lse=None, *,
                             scale=None) -> int:
-        """Bytes of workspace that prefix_attention_dev takes for these arguments (their sizes alone count)."""
-        return self.L.dc_prefix_attention_ws(
+        """Bytes of workspace that prefix_attention_dev takes for these arguments (their sizes alone count).
+        Raises where it would refuse them."""
+        n = self.L.dc_prefix_attention_ws(
             self.h, self._prefix_attn(q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale))
+        if not n and self.L.dc_last_error(self.h):
+            self._check(_lib.DC_E_INVAL, "prefix_attention_ws")
+        return n
 
     def _prefix_attn(self, q, out, k_pre, v_pre, k_own, v_own, lens, lse, scale) -> bytes:
         T = self._types()

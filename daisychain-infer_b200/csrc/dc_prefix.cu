@@ -999,7 +999,11 @@ int run(dc_ctx* ctx, const CUtensorMap (&maps)[4], const PaArgs& a, const Plan& 
 }  // namespace
 
 extern "C" size_t dc_prefix_attention_ws(const dc_ctx* ctx, const dc_prefix_attn* p) {
-  if (!ctx || !p || check(const_cast<dc_ctx*>(ctx), *p) || !p->batch) return 0;
+  if (!ctx) return 0;
+  dc_ctx* c = const_cast<dc_ctx*>(ctx);
+  c->err.clear();  // (a message tells a refusal from a call that needs nothing)
+  if (!p) dc_fail(c, DC_E_INVAL, "prefix_attention: bad arguments");
+  if (!p || check(c, *p) || !p->batch) return 0;
   return ws_bytes_of(make_plan(*p, ctx->sm_count));
 }
 

@@ -242,7 +242,9 @@ int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* a);
  * and sums are f32, the probabilities are rounded to `type` for the product with
  * v.  rows <= 16; head_dim a multiple of 8, <= 128; q, k, v and out rows begin on
  * 16-byte boundaries.  ws: dc_prefix_attention_ws bytes of device memory
- * (16-byte aligned) that no other call uses at the same time. */
+ * (16-byte aligned) that no other call uses at the same time.
+ * dc_prefix_attention_ws answers 0 where nothing is needed, dc_last_error being
+ * empty then, and where it refuses the sizes, types or scale. */
 typedef struct dc_prefix_attn {
   const void *q, *k_pre, *v_pre, *k_own, *v_own;
   const int32_t* lens;

@@ -113,3 +113,17 @@ def test_outputs_that_overlap_themselves_are_refused(P, comp):
     comp.cache_evict_dev(**{**e, "k_out": (both := z(2, 4, 2, 2, 64))[:, :, 0], "v_out": both[:, :, 1]}, budget=4)
     comp.cache_evict_dev(**{**e, "k_out": (both := z(2, 4, 2, 2, 64))[..., 0, :], "v_out": both[..., 1, :]}, budget=4)
     comp.sync()
+
+
+def test_workspace_size_is_refused_as_the_call_is(P, comp):
+    """prefix_attention_ws raises what the call would raise, and is 0 only where nothing is needed."""
+    kv = dict(k_pre=z(5, 2, 64), v_pre=z(5, 2, 64))
+    with pytest.raises(P.DeviceError, match="rows 17"):
+        comp.prefix_attention_ws(z(1, 17, 4, 64), z(1, 17, 4, 64), **kv)
+    with pytest.raises(P.DeviceError, match="scale"):
+        comp.prefix_attention_ws(z(1, 1, 4, 64), z(1, 1, 4, 64), scale=0.0, **kv)
+    assert comp.prefix_attention_ws(z(0, 1, 4, 64), z(0, 1, 4, 64), **kv) == 0
+    assert comp.prefix_attention_ws(z(2, 1, 4, 64), z(2, 1, 4, 64)) == 0
+    with pytest.raises(P.DeviceError, match="rows 17"):
+        comp.prefix_attention_ws(z(0, 17, 4, 64), z(0, 17, 4, 64), **kv)
+    assert comp.prefix_attention_ws(z(2, 1, 4, 64), z(2, 1, 4, 64), **kv) > 0
