@@ -322,6 +322,11 @@ extern "C" int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* p) {
   // (k and v may be interleaved in one buffer)
   if (x.meets(q) || x.meets(k) || x.meets(v) || q.meets(k) || q.meets(v) || !twins_apart(k, v, es_o, dk, dv))
     return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: an output overlaps x or another output");
+  const Span in[4] = {span(A.pos, 4, {{A.axes, A.ld_pos}, {A.rows, 1}}), span(A.kv_heads ? A.slots : nullptr, 8, {{A.rows, 1}}),
+                      span(A.wq, 4, {{A.head_dim, 1}}), span(A.wk, 4, {{A.head_dim, 1}})};
+  for (const Span& i : in)
+    if (i.meets(q) || i.meets(k) || i.meets(v))
+      return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: an output overlaps pos, slots or a norm's weights");
   DeviceGuard g;
   if (int rc = g.enter(ctx)) return rc;
 

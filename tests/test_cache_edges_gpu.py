@@ -127,3 +127,18 @@ def test_workspace_size_is_refused_as_the_call_is(P, comp):
     with pytest.raises(P.DeviceError, match="rows 17"):
         comp.prefix_attention_ws(z(0, 17, 4, 64), z(0, 17, 4, 64), **kv)
     assert comp.prefix_attention_ws(z(2, 1, 4, 64), z(2, 1, 4, 64), **kv) > 0
+
+
+def test_rope_outputs_over_what_it_reads_are_refused(P, comp):
+    """Positions, slots and weights that lie in an output: refused before anything is launched."""
+    before = comp.L.dc_launch_count()
+    t = z(2, 2, 64, t=F32)
+    r = dict(x=z(2, 64 * 4, t=F32), pos=z(2, t=torch.int32), q=t, k=z(2, 1, 64, t=F32), v=z(2, 1, 64, t=F32),
+             slots=z(2, t=torch.int64), wq=z(64, t=F32), wk=z(64, t=F32))
+    for name in ("q", "k", "v"):
+        out = r[name].view(-1)
+        for change in (dict(pos=out[8:10].view(torch.int32)), dict(slots=out[4:8].view(torch.int64)), dict(wq=out[:64]),
+                       dict(wk=out[-64:])):
+            with pytest.raises(P.DeviceError, match="overlaps"):
+                comp.head_norm_rope_dev(**{**r, **change})
+    assert comp.L.dc_launch_count() == before
