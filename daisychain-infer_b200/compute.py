@@ -407,9 +407,10 @@ class Compute:
             if s[-1] != 1 and t.shape[-1] > 1:
                 raise ValueError("cache_evict: the last dimension of every buffer must be contiguous")
             strides += s[:-1]
+        # (a budget beyond the cache keeps all, however large: the library's integers have 32 bits)
         a = _lib.CACHE_EVICT.pack(
             *self._ptrs("cache_evict", k, v, acc, lens, k_out, v_out, acc_out, index, lens_out), *strides,
-            B, kv, D, L, budget, recent, k.element_size())
+            B, kv, D, L, *(max(-1, min(n, 2 ** 31 - 1)) for n in (budget, recent)), k.element_size())
         rc = self.L.dc_cache_evict_dev(self.h, a)
         if rc:
             self._check(rc, "cache_evict")
