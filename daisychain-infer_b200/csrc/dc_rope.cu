@@ -300,8 +300,8 @@ extern "C" int dc_head_norm_rope_dev(dc_ctx* ctx, const dc_head_rope* p) {
   if (!A.x || !A.pos || (A.heads && !A.q) || (A.kv_heads && (!A.k || !A.v)))
     return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: null buffer");
   const int64_t width = (int64_t)(A.heads + 2 * A.kv_heads) * A.head_dim;
-  if ((A.rows > 1 && A.ldx < width) || (A.axes > 1 && A.ld_pos < A.rows))
-    return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: ldx %lld is below a row's %lld, or ld_pos below the rows",
+  if ((A.rows > 1 && A.ldx < width) || (A.axes > 1 && A.ld_pos < 0))  // (ld_pos 0: the same positions on all axes)
+    return dc_fail(ctx, DC_E_INVAL, "head_norm_rope: ldx %lld is below a row's %lld, or ld_pos negative",
                    (long long)A.ldx, (long long)width);
   if (A.kv_heads && (A.cache_seqs < 1 || A.cache_len < 1 || A.cache_seqs > INT64_MAX / A.cache_len ||
                      (!A.slots && A.rows > A.cache_seqs * A.cache_len)))

@@ -142,3 +142,16 @@ def test_rope_outputs_over_what_it_reads_are_refused(P, comp):
             with pytest.raises(P.DeviceError, match="overlaps"):
                 comp.head_norm_rope_dev(**{**r, **change})
     assert comp.L.dc_launch_count() == before
+
+
+def test_rope_with_the_same_positions_on_all_axes(comp):
+    """Text between images has one position on every axis, as an expanded tensor."""
+    g = gen(70)
+    x, pos = normal(g, 5, 6 * 64), torch.arange(5, dtype=torch.int32, device="cuda") * 100
+    got = []
+    for p in (pos.expand(3, 5), pos.expand(3, 5).contiguous()):
+        q, k, v = (z(5, n, 64, t=F32) for n in (4, 1, 1))
+        comp.head_norm_rope_dev(x, p, q, k, v, sections=[16, 8, 8])
+        got.append((q, k, v))
+    comp.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and (got[0][0] != 0).any()
