@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_cache_gpu import BF16, F16, F32, U, attention_ref, check_attention, gen, normal, weights_ref, z
+from test_cache_gpu import BF16, F16, F32, U, attention_ref, check_attention, gen, i32, normal, weights_ref, z
 
 pytestmark = pytest.mark.gpu
 
@@ -82,7 +82,6 @@ def test_outputs_that_overlap_themselves_are_refused(P, comp):
     """Expanded outputs, and values a token behind their keys: refused before anything is launched.  Interleaved
     and permuted ones are taken."""
     before = comp.L.dc_launch_count()
-    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
 
     def refused(call, match):
         with pytest.raises(P.DeviceError, match=match):
@@ -155,3 +154,126 @@ def test_rope_with_the_same_positions_on_all_axes(comp):
         got.append((q, k, v))
     comp.sync()
     assert all(torch.equal(a, b) for a, b in zip(*got)) and (got[0][0] != 0).any()
+
+
+@pytest.mark.parametrize("B", [3, 40], ids=["few rows", "shared"])
+def test_expanded_inputs(comp, B):
+    """Keys and values that all heads or all sequences share, and one query for a batch, as expanded tensors: the
+    bits of their copies."""
+    g = gen(B + 80)
+    H, kv, D, P, L, t = 8, 4, 64, 700, 90, BF16
+    kp, vp = (normal(g, P, 1, D).to(t).expand(P, kv, D) for _ in range(2))
+    ko, vo = (normal(g, 1, L, kv, D).to(t).expand(B, L, kv, D) for _ in range(2))
+    q = normal(g, 1, 2, H, D).to(t).expand(B, 2, H, D)
+    ln = torch.arange(B, dtype=torch.int32, device="cuda") * 5 % 91
+    got = []
+    for same in (lambda x: x, lambda x: x.contiguous()):
+        out, lse = torch.empty(B, 2, H, D, device="cuda"), torch.empty(B, 2, H, device="cuda")
+        comp.prefix_attention_dev(same(q), out, same(kp), same(vp), same(ko), same(vo), ln, lse)
+        acc = torch.zeros(B, kv, L, device="cuda")
+        comp.cache_weights_dev(same(q), same(ko), ln, lse, acc)
+        rows = torch.zeros(1, kv, P, device="cuda")  # (the prefix, against 2 B rows)
+        comp.cache_weights_dev(same(q[:, :1].transpose(0, 1)), same(kp.unsqueeze(0)), i32(P), lse[:, 0].contiguous().unsqueeze(0),
+                               rows, causal=False)
+        got.append((out, lse, acc, rows))
+    comp.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and all((a != 0).any() for a in got[0])
+
+
+@pytest.mark.parametrize("case", [(5, 8, 2, 64, 2000), (50, 32, 8, 128, 300), (3, 15, 5, 64, 40)],
+                         ids=["few rows", "shared", "short"])
+def test_calls_on_two_streams_at_once(P, comp, case):
+    """Two contexts on two streams, calls of all four operators in flight together: the bits of calls one by one."""
+    B, H, kv, D, n = case
+    sides = []
+    for i in range(2):
+        g = gen(90 + i + B)
+        t = BF16
+        s = dict(x=normal(g, B, (H + 2 * kv) * D), pos=torch.arange(B, dtype=torch.int32, device="cuda"),
+                 k=normal(g, B, 200, kv, D).to(t), v=normal(g, B, 200, kv, D).to(t), kp=normal(g, n, kv, D).to(t),
+                 vp=normal(g, n, kv, D).to(t), lens=(torch.arange(B, device="cuda") * 37 % 201).int(),
+                 slots=torch.arange(B, device="cuda") * 200 + 3, acc0=torch.rand(B, kv, 200, generator=g, device="cuda"))
+        s["core"], s["stream"] = P.init_compute(0), torch.cuda.Stream()
+        sides.append(s)
+
+    def calls(s, core):
+        t = BF16
+        q, out, lse = z(B, 1, H, D, t=t), z(B, 1, H, D, t=F32), z(B, 1, H, t=F32)
+        acc = s["acc0"].clone()
+        ko, vo, ao, ix, lo = z(B, 50, kv, D, t=t), z(B, 50, kv, D, t=t), z(B, kv, 50, t=F32), z(B, kv, 50, t=torch.int32), z(
+            B, t=torch.int32)
+        core.head_norm_rope_dev(s["x"], s["pos"], q.view(B, H, D), s["k"], s["v"], slots=s["slots"])
+        core.prefix_attention_dev(q, out, s["kp"], s["vp"], s["k"], s["v"], s["lens"], lse)
+        core.cache_weights_dev(q, s["k"], s["lens"], lse, acc, decay=0.5)
+        core.cache_evict_dev(s["k"], s["v"], acc, s["lens"], ko, vo, ao, ix, lo, budget=50, recent=9)
+        return q, out, lse, acc, ko, vo, ao, ix, lo
+
+    want = [calls(s, comp) for s in sides]
+    torch.cuda.synchronize()
+    for s in sides:
+        s["core"].set_stream(s["stream"])
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s["stream"]):
+                got[i].append(calls(s, s["core"]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for one in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
+        sides[i]["core"].sync()
+        sides[i]["core"].close()
+
+
+def test_offsets_beyond_32_bits(comp):
+    """Tokens 2^24 elements apart in a buffer beyond 2^32: the results of a compact cache, to the bit."""
+    g = gen(99)
+    B, H, kv, D, L, t, far = 2, 8, 2, 64, 150, BF16, 1 << 24
+    whole = torch.empty(B * L * far + far, dtype=t, device="cuda")
+    assert whole.numel() > 1 << 32
+    k, v = (whole.as_strided((B, L, kv, D), (L * far, far, 2 * D, 1), at) for at in (0, D))
+    near = [normal(g, B, L, kv, D).to(t) for _ in range(2)]
+    x, pos = normal(g, 4, (H + 2 * kv) * D), torch.arange(4, dtype=torch.int32, device="cuda")
+    slots = torch.tensor([0, L - 1, L + 7, 2 * L - 1], device="cuda")
+    lens, got = i32(L, L - 3), []
+    for kk, vv in ((k, v), near):
+        kk.copy_(near[0]), vv.copy_(near[1])
+        q = z(4, H, D, t=t)
+        comp.head_norm_rope_dev(x, pos, q, kk, vv, slots=slots)
+        q = q.view(2, 2, H, D)
+        out, lse = torch.empty(B, 2, H, D, device="cuda"), torch.empty(B, 2, H, device="cuda")
+        comp.prefix_attention_dev(q, out, kk[1], vv[1], kk, vv, lens, lse)
+        acc = torch.zeros(B, kv, L, device="cuda")
+        comp.cache_weights_dev(q, kk, lens, lse, acc)
+        many = torch.zeros(1, kv, L, device="cuda")
+        comp.cache_weights_dev(q.view(1, 4, H, D).repeat(1, 20, 1, 1), kk[1:], i32(L),
+                               lse.view(1, 4, H).repeat(1, 20, 1), many, causal=False)
+        ko, vo = z(B, 40, kv, D, t=t), z(B, 40, kv, D, t=t)
+        outs = (z(B, kv, 40, t=F32), z(B, kv, 40, t=torch.int32), i32(0, 0))
+        comp.cache_evict_dev(kk, vv, acc, lens, ko, vo, *outs, budget=40, recent=5)
+        got.append((q, out, lse, acc, many, ko, vo, *outs, kk.clone(), vv.clone()))
+    comp.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_eviction_to_offsets_beyond_32_bits(comp):
+    """Kept tokens and their weights and places, as far apart."""
+    g = gen(100)
+    B, kv, D, L, t, far = 1, 2, 64, 300, BF16, 1 << 24
+    k, v = (normal(g, B, L, kv, D).to(t) for _ in range(2))
+    acc = torch.rand(B, kv, L, generator=g, device="cuda")
+    whole = torch.empty(140 * far, dtype=t, device="cuda")
+    words = torch.empty((1 << 32) + 512, dtype=torch.int32, device="cuda")
+    got = []
+    for wide in (True, False):
+        if wide:
+            ko, vo = (whole.as_strided((B, 130, kv, D), (130 * far, far, 2 * D, 1), at) for at in (0, D))
+            ix, ao = words[:(1 << 31) + 256], words[(1 << 31) + 256:].view(F32)
+            ix, ao = (b.as_strided((B, kv, 130), (1 << 31, 1 << 31, 1)) for b in (ix, ao))
+        else:
+            ko, vo, ix, ao = z(B, 130, kv, D, t=t), z(B, 130, kv, D, t=t), z(B, kv, 130, t=torch.int32), z(B, kv, 130, t=F32)
+        lo = i32(0)
+        comp.cache_evict_dev(k, v, acc, i32(L), ko, vo, ao, ix, lo, budget=130, recent=20)
+        got.append((ko.clone(), vo.clone(), ao.clone(), ix.clone(), lo))
+    comp.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
