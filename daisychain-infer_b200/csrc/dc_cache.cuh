@@ -43,9 +43,12 @@ struct DeviceGuard {
   }
 };
 
-// One launch on the context's stream, in clusters of `cluster` blocks along x,
-// as a programmatic dependent of what runs before: every kernel here executes
-// griddepcontrol.wait before it touches memory.
+// One launch on the context's stream, in clusters of `cluster` blocks along x, as a
+// programmatic dependent of what runs before: it may begin while that still runs, so a
+// kernel executes griddepcontrol.wait before it touches memory.  The exceptions are
+// k_own and k_join of dc_prefix.cu where they are launched `behind` the kernel of the
+// same call before them; the comments there say which earlier wait covers what they
+// touch and which later one their end.  They may follow no other kernel in that form.
 template <typename... P, typename... A>
 static int launch(dc_ctx* ctx, void (*kern)(P...), dim3 grid, int threads, int smem, int cluster, const A&... args) {
   if (int rc = dc_set_smem(ctx, (const void*)kern, smem)) return rc;

@@ -113,16 +113,18 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // + 500, shared memory 512 + 256 for their operands and 256 for the copies: with
 // 64-key tiles in two smaller blocks an SM the operands and copies alone took 1536.
 // Measured: 76 us for 256 rows of each of 8 heads on 65536 keys of 128 channels
-// (0.9 PFLOP/s, 3.5 TB/s), about 3700 cycles for a tile of both groups.  Neither
-// unit is what it waits for (the exponential unit is busy 39% of the time, at 64
-// channels 51%; the tensor pipe 45%): with no exponentials and an eighth of the
+// (0.9 PFLOP/s, 3.5 TB/s; with the join), about 3700 cycles for a tile of both groups.
+// Neither unit is what it waits for (the exponential unit is busy 37% of the time, at
+// 64 channels 51%; the tensor pipe 43%): with no exponentials and an eighth of the
 // products it still takes 60.  That is a group's chain of score, load, maximum,
 // probabilities, store and product, which two groups fill only in part.  Twice the
 // warps a group, rolled loops, the maximum of the tile before, a forced
 // order of the groups and an issuing warp for each kind of product gave nothing or
 // lost; scores of 64 keys, two buffers a group, one being formed under the other's
 // softmax, took 106 us for 64 sequences over 65536 keys where this takes 100 (and 53
-// for 56 on 24 x 5 drafts of 64 channels); there is no TMEM for a third group.
+// for 56 on 24 x 5 drafts of 64 channels); there is no TMEM for a third group.  (What
+// is compared here was measured before double waits ordered the warp's memory, which
+// made 100 us 101, 56.5 us 57.6 and 28.4 us, 32 sequences over 8192 keys, 28.9.)
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
 constexpr int SH_THREADS = 384;
@@ -179,7 +181,6 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
   const int n = (k1 - k0 + KEYS - 1) / KEYS;
   const bool two = 2 * pair + 1 < a.pre_m;  // two tiles of rows
   // tiles of keys: all for both groups, or every other
-  const int stride = two ? 1 : 2;
   const int count0 = two ? n : (n + 1) / 2, count1 = two ? n : n / 2;
 
   if (threadIdx.x == 0) {

@@ -6,20 +6,24 @@
 //     lo' = lo cos t - hi sin t,  hi' = hi cos t + lo sin t,  (lo, hi) = (y[i], y[i + rot/2])
 // queries to their own buffer, keys and values to their cache slots.
 //
-// Bound by HBM: every element is read once and written once, so nothing is
-// staged.  A head belongs to hd/8 neighbouring lanes; a lane holds four
-// channels i.. and their partners i + rot/2.., so the rotation needs no
+// Every element is read once and written once, so nothing is staged.  A head
+// belongs to hd/16 neighbouring lanes (hd/8 where rows are not aligned); a lane holds
+// eight (four) channels i.. and their partners i + rot/2.., so the rotation needs no
 // exchange and the norm one shuffle tree, and a warp walks a row's heads with
 // the lane's angles in registers: the angle in turns (position x frequency / 2
 // pi) in 64 bits, where a position of a million still has 33 bits behind the
 // point, its fraction rounded to f32 for sincospi.
 //
-// Measured: 2048 rows of 32 + 2 x 8 heads of 128, f32 to bf16, 22.7 us (75 MB, 3.3
-// TB/s); 10007 rows of 32 + 2 x 4 heads of 64, f16, three axes, 28.6 us (103 MB, 3.6
-// TB/s); 32 rows 3 us.  What keeps it from HBM's rate is how little is in flight:
-// 16 warps an SM, each a row's load, a norm's shuffles and a store in turn.  Loads
-// through shared memory (24.7 and 29.7 us) and a whole row an item (20.0 and 33.0)
-// were no better for both.
+// Measured: 2048 rows of 32 + 2 x 8 heads of 128, f32 to bf16, 23.0 us (75 MB, 3.3
+// TB/s); 10007 rows of 32 + 2 x 4 heads of 64, f16, three axes, 28.9 us (103 MB, 3.6
+// TB/s); 32 rows 3.2 us.  What keeps it from HBM's rate is how little is in flight,
+// and that is this form's choice: three or four heads a lane at 128 registers (the
+// f32 variants spill 12 bytes) leave 16 warps an SM, a warp asks for the next item only
+// when it is done with one (load, angles, norm, store), items are uneven (a row's
+// last one may hold a single step of four and waits as long), and an f32 lane's two
+// 16-byte loads each touch half of a sector.  Loads through shared memory by each lane
+// (24.7 and 29.7 us where this took 22.7 and 28.6) and a whole row an item (20.0 and
+// 33.0) were no better for both; bulk copies into a ring have not been tried.
 #include <math.h>
 
 #include <algorithm>

@@ -11,7 +11,11 @@
 //
 // k_weights_few, up to 128 columns: a block keeps Q in shared memory and streams
 // its share of the cache's keys (16 KB panels through a ring by TMA), two blocks an
-// SM, scores double-buffered in TMEM.  HBM-bound: each key is read once.
+// SM, scores double-buffered in TMEM.  HBM-bound: each key is read once.  The shares
+// are of the cache's size, since the lengths are known on the device alone: 16
+// sequences of 8 heads and 8192 keys take 49 us (5.6 TB/s) where all are full and 44
+// (4.7 TB/s) with lengths from half to all, the fullest SM then having 1.5 times the
+// mean.
 //
 // k_weights_many: a block keeps 128 keys in TMEM, as the first operand, and streams
 // Q tiles (out of L2) past them, half a tile's scores (64 columns) in each of three
@@ -19,9 +23,10 @@
 // exponential warps an SM: the unit takes 16 a cycle and SM, 448 cycles a half tile
 // with one pair in eight on the multiply-add pipe, but a warp's loads, waits and
 // sums around 32 exponentials a thread take as long, and only other warps fill
-// them.  1024 rows of 32 heads over 16384 keys of 8: 185 us, 0.72 PFLOP/s (the
-// unit alone 117); with 64 columns a warp and half as many warps 214, with 256 keys
-// a block and two groups of four warps 228.
+// them.  1024 rows of 32 heads over 16384 keys of 8: 190 us, 0.70 PFLOP/s (the
+// unit alone 117).  It was 185 before double waits ordered the warp's memory (188) and
+// rows of lse -inf were passed over (190); then, with 64 columns a warp and half as
+// many warps, 214, with 256 keys a block and two groups of four warps 228.
 //
 // One warp copies, one issues the products.  Every wait is bounded; a block whose
 // wait gives up waits for the copies and products that it has in flight (bounded as
@@ -264,8 +269,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
 
 // Blocks of 128 keys against all Q tiles, two an SM, a half tile (64 columns) at a
 // time.  TMEM columns: the keys (64 x 32 bits a lane), three half tiles' scores.
-// (One pair in eight by multiply-adds: 185 us as above; in six 186, in twelve 192,
-// in four 200, none 196.)
+// (One pair in eight by multiply-adds: 185 us, then; in six 186, in twelve 192, in
+// four 200, none 196.)
 constexpr int HALF = COLS / 2, BUFS = 3, SCALES = 4;
 constexpr int MANY_THREADS = 352, MMA_WARP = 0, TMA_WARP = 1, SCALE_WARP = 2, EXP_WARP = 3;
 constexpr uint32_t s_col(int i) { return 64 + i * HALF; }
