@@ -17,7 +17,14 @@
 // exact there as below 1.  f16 ends at 2^16 and has no normal numbers below 2^-14, so
 // there they are formed 2^7 larger, up to 2^15: what is lost of a key far below the
 // maximum is at most 2^-32 of it (2^-25 unshifted, and then a few hundred keys 2^-26
-// below a dominant one vanished from out, though not from lse).
+// below a dominant one vanished from out, though not from lse).  Parts are stored
+// without that factor.
+//
+// An exponent is c x - m with m = c times the maximum, one multiply-add; the rounding
+// of m then shifts all of a row's alike.  Where the maximum is so far from 0 that this
+// would show (FAR), and in k_own, which has instructions to spare, it is c times the
+// difference to the maximum: with scores of 10^9 and more the product's rounding alone
+// passed what f32 exponents hold, and finite scores gave NaN.
 //
 // Rows of one sequence may see different last tokens (rows > 1).  k_own takes
 // only the tokens that all rows see; the up to rows - 1 behind them go to k_join,
@@ -34,6 +41,7 @@
 // waits for the copies and products that it has in flight (bounded as well) and ends,
 // its part without weight, and dc_sync reports it.
 #include <algorithm>
+#include <type_traits>
 
 #include "dc_cache.cuh"
 #include "dc_ring.h"
@@ -47,12 +55,12 @@ using dcu::F2;
 constexpr int MAX_ROWS = 16;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RAISE = 8.0f;  // growth of a row's maximum (in powers of two) that rescales it
-constexpr float F16_UP = 7.0f;  // powers of two by which f16 probabilities are larger
-// What is taken off a row's exponents where its maximum is mx (a part's m).
+constexpr float FAR = 4096.0f;  // of a maximum times c
+// Powers of two by which f16 probabilities are larger, and the factor that takes it back.
 template <bool BF16>
-__device__ __forceinline__ float base_of(float mx, float c) {
-  return fmaf(mx, c, BF16 ? 0.0f : -F16_UP);
-}
+constexpr float UP = BF16 ? 0.0f : 7.0f;
+template <bool BF16>
+constexpr float DOWN = BF16 ? 1.0f : 0.0078125f;
 
 struct PaArgs {
   const void *q, *k_own, *v_own;
@@ -123,8 +131,9 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* x, uint32_t px, uint64_t* y
 // lost; scores of 64 keys, two buffers a group, one being formed under the other's
 // softmax, took 106 us for 64 sequences over 65536 keys where this takes 100 (and 53
 // for 56 on 24 x 5 drafts of 64 channels); there is no TMEM for a third group.  (What
-// is compared here was measured before double waits ordered the warp's memory, which
-// made 100 us 101, 56.5 us 57.6 and 28.4 us, 32 sequences over 8192 keys, 28.9.)
+// is compared here was measured before double waits ordered the warp's memory and far
+// scores had their own form: 100 us are 102 now, 56.5 are 57.7, and 28.4, of 32
+// sequences over 8192 keys, 29.2.)
 constexpr int ROWS = 128;  // query rows of a group: the MMA's M
 constexpr int KEYS = 128;  // keys of a tile
 constexpr int SH_THREADS = 384;
@@ -319,7 +328,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     const bool used = quarter * 32 < nrows;  // (a warp without rows only keeps the barriers going)
     const int count = g ? count1 : count0;
     float mx = -INFINITY, l = 0.0f;  // the maximum in use (scores before c), the sum
-    bool ok = true;
+    bool ok = true, far = false;     // (far: for a row of this warp)
     for (int j = 0; j < count; j++) {
       if (!dcu::warp_wait(&s_full[g], j & 1, a.status)) { ok = false; break; }
       dcu::fence_after();
@@ -353,8 +362,10 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
 #pragma unroll
           for (int x = 0; x < 4; x++) m4[x] = dcu::max3(m4[x], __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
         const float top = fmaxf(dcu::max3(m4[0], m4[1], m4[2]), m4[3]);
+        const auto is_far = [&] { return __any_sync(~0u, mx != -INFINITY && fabsf(mx) * a.c > FAR); };
         if (j == 0) {
           mx = top;
+          far = is_far();
         } else if (__any_sync(~0u, top > mx && !((top - mx) * a.c <= RAISE))) {
           // O *= 2^(c (old - new)), once it holds the product of the tile before
           // (the next product needs these probabilities)
@@ -363,6 +374,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           const float up = fmaxf(mx, top);
           const float f = mx == -INFINITY ? 0.0f : mx == up ? 1.0f : dcu::ex2((mx - up) * a.c);
           mx = up;
+          far = is_far();
           l *= f;
 #pragma unroll 1
           for (int col = 0; col < C::WIDTH; col += 16) {
@@ -375,44 +387,67 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           }
           dcu::wait_st();
         }
-        const float base = mx == -INFINITY ? 0.0f : base_of<BF16>(mx, a.c);
-        b2 = dcu::f2(-base, -base);
+        const float m = mx == -INFINITY ? 0.0f : mx;
+        float b = fmaf(m, -a.c, UP<BF16>);
+        if (far && C::APART) {
+          b = UP<BF16>;
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int y = 0; y < 32; y++) s[x][y] = __float_as_uint(__uint_as_float(s[x][y]) - m);
+        } else if (far) {
+          b = -m;
+        }
+        b2 = dcu::f2(b, b);
       }
       bool met = true;
+      auto exponentials = [&](auto is_far) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        // (a warp without rows waits too: its arrival belongs to this tile's phase)
-        if (C::APART && !used && half == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
-        if (used) {
+        for (int half = 0; half < 2; half++) {
+          // (a warp without rows waits too: its arrival belongs to this tile's phase)
+          if (C::APART && !used && half == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
+          if (used) {
 #pragma unroll
-          for (int x = 2 * half; x < 2 * half + 2; x++) {
-            uint32_t p[16];
+            for (int x = 2 * half; x < 2 * half + 2; x++) {
+              uint32_t p[16];
 #pragma unroll
-            for (int y = 0; y < 16; y++) {
-              // (the sum keeps the unrounded values: lse is exact to f32; P is
-              // rounded to the type of the products' operands, half a step each)
-              F2 e = dcu::fma2(dcu::f2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), c2, b2);
-              if (y % C::FMA_EVERY == C::FMA_EVERY - 1) {
-                e = dcu::ex2_fma(e);
-              } else {
+              for (int y = 0; y < 16; y++) {
+                // (the sum keeps the unrounded values: lse is exact to f32; P is
+                // rounded to the type of the products' operands, half a step each)
+                F2 e = dcu::f2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1]));
+                if constexpr (decltype(is_far)::value)
+                  e = dcu::fma2(dcu::add2(e, b2), c2, dcu::f2(UP<BF16>, UP<BF16>));
+                else
+                  e = dcu::fma2(e, c2, b2);
+                if (y % C::FMA_EVERY == C::FMA_EVERY - 1) {
+                  e = dcu::ex2_fma(e);
+                } else {
+                  const float2 v = dcu::split(e);
+                  e = dcu::f2(dcu::ex2(v.x), dcu::ex2(v.y));
+                }
+                sum[y & 1] = dcu::add2(sum[y & 1], e);
                 const float2 v = dcu::split(e);
-                e = dcu::f2(dcu::ex2(v.x), dcu::ex2(v.y));
+                p[y] = pack2<BF16>(v.x, v.y);
               }
-              sum[y & 1] = dcu::add2(sum[y & 1], e);
-              const float2 v = dcu::split(e);
-              p[y] = pack2<BF16>(v.x, v.y);
+              // (beside the scores: where the product of the tile before has read the ones there)
+              if (C::APART && x == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
+              dcu::fence_after();
+              dcu::st16(p_at + x * 16, p);
             }
-            // (beside the scores: where the product of the tile before has read the ones there)
-            if (C::APART && x == 0 && j > 0) met = dcu::warp_wait(&o_done[g], (j - 1) & 1, a.status);
-            dcu::fence_after();
-            dcu::st16(p_at + x * 16, p);
+            dcu::wait_st();
           }
-          dcu::wait_st();
+          dcu::fence_before();
+          __syncwarp();
+          if (lane == 0) dcp::mbar_arrive(&p_ready[2 * g + half]);
         }
-        dcu::fence_before();
-        __syncwarp();
-        if (lane == 0) dcp::mbar_arrive(&p_ready[2 * g + half]);
-      }
+      };
+      // (far scores in a loop of their own: taking m off beforehand cost 64 x 65536 3 us in
+      // spilled registers; where that costs nothing, at 64 channels, a second loop cost
+      // the drafts 2.5)
+      if (far && !C::APART)
+        exponentials(std::true_type());
+      else
+        exponentials(std::false_type());
       const float2 both = dcu::split(dcu::add2(sum[0], sum[1]));
       l += both.x + both.y;
       if (!met) { ok = false; break; }
@@ -427,7 +462,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
     uint8_t* mine = ring + (g * 128 + row) * STRIDE;
     ok = ok && count > 0 && used && dcu::warp_wait(&o_done[g], (count - 1) & 1, a.status);
     if (!ok) mx = -INFINITY, l = 0.0f;
-    float2 ml = make_float2(mx == -INFINITY ? -INFINITY : base_of<BF16>(mx, a.c), l);
+    float2 ml = make_float2(mx == -INFINITY ? -INFINITY : mx * a.c, DOWN<BF16> * l);
     dcp::named_sync(1, 256);
     dcu::fence_after();
     // this row, times f, and (join) the second group's, times f_other; a factor of
@@ -472,7 +507,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1)
           f_other = x.y == 0.0f ? 0.0f : dcu::ex2(x.x - base);
           ml = make_float2(top, fmaf(f_other, x.y, f * ml.y));
         }
-        put(!two, f, f_other);
+        put(!two, f * DOWN<BF16>, f_other * DOWN<BF16>);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (row < nrows)
           asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + part * C::WIDTH),
@@ -686,15 +721,13 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
             for (int y = 0; y < 4; y++) o[x][y] *= f[y >> 1];
         }
       }
-      float base[2];
-#pragma unroll
-      for (int y = 0; y < 2; y++) base[y] = mx[y] == -INFINITY ? 0.0f : base_of<BF16>(mx[y], a.c);
+      const float m[2] = {mx[0] == -INFINITY ? 0.0f : mx[0], mx[1] == -INFINITY ? 0.0f : mx[1]};
       float e[2][4];
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
         for (int y = 0; y < 4; y++) {
-          e[x][y] = dcu::ex2(fmaf(s[x][y], a.c, -base[y >> 1]));
+          e[x][y] = dcu::ex2(fmaf(s[x][y] - m[y >> 1], a.c, UP<BF16>));
           l[y >> 1] += e[x][y];
         }
       const uint32_t p[4] = {pack2<BF16>(e[0][0], e[0][1]), pack2<BF16>(e[0][2], e[0][3]), pack2<BF16>(e[1][0], e[1][1]),
@@ -724,11 +757,11 @@ __global__ void __launch_bounds__(OWN_WARPS * 32, 2)
       const int row = lane / 4 + 8 * y;
       if (lane % 4 == 0)
         *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + C::WIDTH) =
-            make_float2(mx[y] == -INFINITY ? -INFINITY : base_of<BF16>(mx[y], a.c), l[y]);
+            make_float2(mx[y] == -INFINITY ? -INFINITY : mx[y] * a.c, DOWN<BF16> * l[y]);
 #pragma unroll
       for (int x = 0; x < 8 * NP; x++)
         *reinterpret_cast<float2*>(mine + row * (C::WIDTH + 4) + 8 * x + 2 * (lane % 4)) =
-            make_float2(o[x][2 * y], o[x][2 * y + 1]);
+            make_float2(DOWN<BF16> * o[x][2 * y], DOWN<BF16> * o[x][2 * y + 1]);
     }
     __syncthreads();
     for (int j = threadIdx.x; j < nrows * (C::WIDTH / 4); j += OWN_WARPS * 32) {

@@ -277,3 +277,62 @@ def test_eviction_to_offsets_beyond_32_bits(comp):
         got.append((ko.clone(), vo.clone(), ao.clone(), ix.clone(), lo))
     comp.sync()
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("B, heads", [(3, 4), (40, 2), (40, 150), (200, 130)],
+                         ids=["few rows", "shared", "many tiles", "two tiles of rows"])
+@pytest.mark.parametrize("t, q0, k0", [(F16, 2.0 ** 4, 2.0 ** 15), (F16, 2.0 ** 10, 2.0 ** 15), (F16, 2.0 ** 15, 2.0 ** 15),
+                                       (F16, -2.0 ** 15, 2.0 ** 15), (BF16, 2.0 ** 20, 2.0 ** 14), (BF16, 2.0 ** 50, 2.0 ** 50),
+                                       (BF16, -2.0 ** 50, 2.0 ** 50)], ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_far_scores(comp, D, t, q0, k0, B, heads):
+    """Scores far from 0, as exact products of one channel: those of the largest are equal, the next lies 2^-4 of it
+    below, so each row is the mean of the values that have the largest, off by the roundings of
+    the probabilities (equal ones: none), the output (f32) and a sum of up to 1024 terms, and lse is the largest to f32."""
+    g = gen(B + heads)
+    P, L, R = 700, 90, 2
+    pick = torch.randint(0, 6, (P + L,), generator=g, device="cuda")
+    pick[3], pick[P + 5] = 5, 5  # (each cache has the largest, the first two drafts' common tokens too)
+    value = torch.tensor([1.0, 1.125, 1.25, 1.5, 1.75, 1.875], device="cuda")[pick] * k0
+    if q0 < 0:  # (the largest score is then the one nearest to 0, below it)
+        value = torch.where(pick == 5, 1.0 * k0, value * 1.0625)
+    k, v = z(P + L, heads, D, t=t), normal(g, P + L, heads, D).to(t)
+    k[..., 0] = value.to(t).view(-1, 1)
+    q = z(B, R, heads, D, t=t)
+    q[..., 0] = q0
+    ko, vo = (x[P:].unsqueeze(0).expand(B, L, heads, D).contiguous() for x in (k, v))
+    out, lse = torch.empty(B, R, heads, D, device="cuda"), torch.empty(B, R, heads, device="cuda")
+    comp.prefix_attention_dev(q, out, k[:P], v[:P], ko, vo, torch.full((B,), L, dtype=torch.int32, device="cuda"), lse,
+                              scale=1.0)
+    comp.sync()
+    for r in range(R):
+        seen = P + L - (R - 1 - r)
+        x = k[:seen, 0, 0].double() * q0
+        best = x == x.max()
+        want = v[:seen][best].double().mean(0)
+        size = v[:seen][best].double().abs().mean(0)
+        assert ((out[:, r].double() - want).abs() <= (2 * 1024 * U[F32] + 4 * U[F32]) * size).all()
+        top = float(x.max()) + math.log(int(best.sum()))
+        assert ((lse[:, r].double() - top).abs() <= 8 * U[F32] * abs(top)).all()
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, kv", [(4, 296), (40, 128), (200, 128)], ids=["few rows", "one tile of rows", "two"])
+def test_attention_of_near_and_far_rows(comp, B, kv, D, t):
+    """Rows whose scores end anywhere from 6 to 12000, side by side, and grow from tile to tile: a row's
+    maximum passes where the exponents are formed in another way while its neighbours' do not."""
+    g = gen(B + D)
+    P = 1100
+    kp, vp = z(P, kv, D, t=t), normal(g, P, kv, D).to(t)
+    kp[..., 0] = (torch.linspace(-300, 375, P, device="cuda") + torch.randn(P, generator=g, device="cuda")).to(t).view(P, 1)
+    q = z(B, 1, kv, D, t=t)
+    q[..., 0] = (32 * 0.5 ** (torch.arange(B, device="cuda") % 12)).to(t).view(B, 1, 1)
+    out, lse = torch.empty(B, 1, kv, D, device="cuda"), torch.empty(B, 1, kv, device="cuda")
+    comp.prefix_attention_dev(q, out, kp, vp, lse=lse, scale=1.0)
+    comp.sync()
+    n = min(B, 12)
+    ref = attention_ref(q[:n], kp, vp, None, None, None, 1.0)
+    for b in range(0, B, n):
+        m = min(n, B - b)
+        check_attention(out[b:b + m], lse[b:b + m], tuple(x[:m] for x in ref), t, float(vp.abs().max()))
