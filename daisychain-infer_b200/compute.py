@@ -215,9 +215,9 @@ class Compute:
         (int64; a negative one is padding and writes neither; None: row i at slot
         i).  Slots count through the sequences, and no two rows of a call share one.
         wq, wk (head_dim, f32): the norm's weights, None for no norm.  pos int32,
-        (rows,) or (axes, rows); sections: pairs of channels that each axis turns,
-        in runs, or with cyclic by turns (pair i on axis i % axes).  rot: channels
-        that are rotated (all); inv_freq (host f64, rot/2) in place of theta.
+        (rows,) or (axes, rows), an expanded row too; sections: pairs of channels that
+        each axis turns, in runs, or with cyclic by turns (pair i on axis i % axes).
+        rot: channels that are rotated (all); inv_freq (host f64, rot/2) in place of theta.
         A slot behind the cache is not written and makes the next sync() raise."""
         T = self._types()
         if x.ndim != 2 or q.ndim != 3 or k.ndim not in (3, 4) or v.shape != k.shape:
@@ -348,7 +348,7 @@ class Compute:
         prefix_attention_dev takes and gives them (with a prefix, lse spans both).
         causal: row r sees lens[b] - (rows - 1 - r) tokens; False: all rows see all
         (the shared prefix: its k as one sequence, all rows of the batch as rows).
-        decay 0 overwrites."""
+        decay 0 overwrites; a row of lse -inf (padding) adds nothing, whatever q holds there."""
         T = self._types()
         dt = q.dtype
         if q.ndim != 4 or k.ndim != 4 or k.dtype is not dt or dt not in T:

@@ -202,7 +202,8 @@ int dc_rmsnorm_dev(dc_ctx* ctx, const float* x, int rows, int cols, const float*
  * normalised, y = x / sqrt(mean(x^2) + eps) * w (skipped where wq / wk is
  * NULL), and its first `rot` channels are rotated: with (lo, hi) = (y[i],
  * y[i + rot/2]) and the angle t_i = position * theta^(-2i/rot), lo' = lo cos t -
- * hi sin t, hi' = hi cos t + lo sin t.  Positions are pos[axis * ld_pos + row];
+ * hi sin t, hi' = hi cos t + lo sin t.  Positions are pos[axis * ld_pos + row]
+ * (ld_pos 0: the same on every axis);
  * pair i takes the axis that `sections` gives it (sections[0..axes) pairs, rot/2
  * in all): runs in order of the axes, or (cyclic = 1) pair i the axis i % axes
  * while i / axes < sections[i % axes], else axis 0.  inv_freq (host, rot/2
@@ -266,8 +267,8 @@ int dc_prefix_attention_dev(dc_ctx* ctx, const dc_prefix_attn* a, void* ws, size
  * causal = 1: row r sees tokens j < lens[b] - (rows - 1 - r), as above; 0: all
  * rows see all tokens (a shared prefix: batch 1, the batch's rows as rows).
  * decay (rounded to f32) = 0 overwrites without reading acc; a row of lse -inf
- * adds nothing.  The sum's order is fixed: equal inputs give equal bits.  Types
- * and alignment as above; heads / kv_heads <= 128. */
+ * adds nothing, whatever its queries hold.  The sum's order is fixed: equal inputs
+ * give equal bits.  Types and alignment as above; heads / kv_heads <= 128. */
 typedef struct dc_cache_weight {
   const void *q, *k;
   const int32_t* lens;
